@@ -17,16 +17,21 @@ from __future__ import annotations
 
 from . import _lib
 from .packers.fp8 import PackedFP8, pack_fp8_tensor, unpack_fp8_tensor
+from .packers.mxfp4 import pack_mxfp4_tensor, unpack_mxfp4_tensor
 from .routines.dot import (dot_fp8_acc_fp32_gpu, dot_fp8_e4m3_acc_fp32_gpu,
                            dot_fp8_e5m2_acc_fp32_gpu)
 from .routines.gemv import (gemv_fp8_acc_fp32_gpu, gemv_fp8_e4m3_acc_fp32_gpu,
                             gemv_fp8_e5m2_acc_fp32_gpu, gemv_fp8_multi_acc_fp32_gpu,
                             gemv_fp8_ret_packed_gpu)
+from .routines.gemm import gemm_mxfp4_acc_fp32_gpu, gemv_mxfp4_acc_fp32_gpu
+from .routines.rotary import rotary_frequencies, rotary_gpu
 
 __version__ = "0.2.0"
 __all__ = ["pack_fp8_tensor", "unpack_fp8_tensor", "gemv", "dot", "PackedFP8", "device_status",
            "gemv_fp8_acc_fp32_gpu", "gemv_fp8_e5m2_acc_fp32_gpu", "gemv_fp8_e4m3_acc_fp32_gpu",
-           "gemv_fp8_ret_packed_gpu", "gemv_fp8_multi_acc_fp32_gpu", "dot_fp8_acc_fp32_gpu", "dot_fp8_e5m2_acc_fp32_gpu", "dot_fp8_e4m3_acc_fp32_gpu"]
+           "gemv_fp8_ret_packed_gpu", "gemv_fp8_multi_acc_fp32_gpu", "dot_fp8_acc_fp32_gpu", "dot_fp8_e5m2_acc_fp32_gpu", "dot_fp8_e4m3_acc_fp32_gpu",
+           "pack_mxfp4_tensor", "unpack_mxfp4_tensor", "gemv_mxfp4_acc_fp32_gpu", "gemm_mxfp4_acc_fp32_gpu",
+           "rotary_frequencies", "rotary_gpu"]
 
 
 def _mode_of(mode, *operands) -> str:

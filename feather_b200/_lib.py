@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_PKG, "libfeather_b200_debug.so" if os.environ.get("FEAT
                         else "libfeather_b200.so")
 
 MODE_IDS = {"E5M2": 0, "E4M3": 1}
-SRC_F16, SRC_F32 = 0, 1
+SRC_F16, SRC_F32, SRC_BF16, SRC_MXFP4 = 0, 1, 2, 3
 DECODE_KERNEL, DECODE_IEEE = 0, 1
 
 # every symbol include/feather_b200.h declares: name -> (restype, argtypes)
@@ -57,6 +57,12 @@ SYMBOLS = {
     "feather_dot_workspace_bytes": (_i64, [_i64]),
     "feather_dot_fp8_static": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp]),
     "feather_dot_fp8_static_max_words": (_i64, []),
+    "feather_encode_mxfp4": (_i32, [_vp, _i32, _vp, _vp, _i64, _i64, _vp]),
+    "feather_decode_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _vp]),
+    "feather_gemv_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "feather_gemm_mxfp4": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp]),
+    "feather_rotary": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32,
+                              ctypes.c_float, _vp]),
 }
 
 

@@ -21,6 +21,10 @@
 #include "gemv_multi_tc.cuh"
 #include "gemv_mma.cuh"
 #include "gemv_ring.cuh"
+#include "mxfp4_codec.cuh"
+#include "mxfp4_gemm.cuh"
+#include "mxfp4_gemv.cuh"
+#include "rotary.cuh"
 
 namespace feather {
 
@@ -850,6 +854,158 @@ static int dot_static_launch(const uint32_t* a, const uint32_t* b, float* out, l
     return dot_launch_any<MODE>(a, b, out, ticket, partial, n_words, kStaticDotSlots, dev, s);
 }
 
+// ------------------------------------------- microscaled 4-bit, rotary ------
+// Limits of the microscaled entry points: a row's blocks and the rows are counted in 32 bits.
+constexpr long long kMxMaxCols = 1ll << 30, kMxMaxRows = 1ll << 31;
+static inline int mx_blocks(long long cols) { return (int)((cols + kMxBlock - 1) / kMxBlock); }
+
+// A grid of 256-thread CTAs for `units` pieces of work per warp: as many as there are, at most
+// 32 CTAs per SM (the streaming kernels above measured best there).
+static unsigned stream_grid(long long units, const DeviceInfo& dev) {
+    const long long ctas = (units + 7) / 8, most = 32ll * dev.sm_count;
+    return (unsigned)(ctas < 1 ? 1 : ctas < most ? ctas : most);
+}
+
+template <int T>
+static int mx_encode_launch(const void* src, unsigned char* codes, unsigned char* scales, long long rows, long long cols,
+                            const DeviceInfo& dev, cudaStream_t s) {
+    if (cols % kMxBlock == 0 && aligned(src, 16)) {
+        const long long words = rows * (cols / 8);
+        mx_encode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
+            src, reinterpret_cast<uint32_t*>(codes), scales, words);
+    } else {
+        const int blocks = mx_blocks(cols);
+        mx_encode_ragged_kernel<T><<<stream_grid(rows * blocks, dev), 256, 0, s>>>(
+            reinterpret_cast<const typename MxElem<T>::type*>(src), reinterpret_cast<uint32_t*>(codes), scales, rows,
+            cols, blocks);
+    }
+    return launch_status();
+}
+
+template <int T>
+static int mx_decode_launch(const unsigned char* codes, const unsigned char* scales, void* dst, long long rows,
+                            long long cols, const DeviceInfo& dev, cudaStream_t s) {
+    if (cols % kMxBlock == 0 && aligned(dst, 16)) {
+        const long long words = rows * (cols / 8);
+        mx_decode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
+            reinterpret_cast<const uint32_t*>(codes), scales, dst, words);
+    } else {
+        const int blocks = mx_blocks(cols);
+        mx_decode_ragged_kernel<T><<<stream_grid(rows * blocks, dev), 256, 0, s>>>(
+            codes, scales, reinterpret_cast<typename MxElem<T>::type*>(dst), rows, cols, blocks);
+    }
+    return launch_status();
+}
+
+template <int VT, int P, int R>
+static int mx_gemv_launch(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
+    auto kernel = mx_gemv_kernel<VT, P, R>;
+    a.chunk_blocks = kMgVecHalfs / (2 * P) / kMxBlock & ~3;
+    if (a.blocks < a.chunk_blocks) a.chunk_blocks = (a.blocks + 3) & ~3;
+    const int most = mg_smem_bytes<P>(kMgVecHalfs / (2 * P) / kMxBlock & ~3, 2 * P);
+    static std::atomic<unsigned long long> configured{0};
+    if (int st = ensure_smem(kernel, most, configured)) return st;
+    const int tiles = ((a.blocks < a.chunk_blocks ? a.blocks : a.chunk_blocks) + 3) / 4;
+    a.col_warps = kMgWarps;
+    while (a.col_warps > 1 && a.col_warps > tiles) a.col_warps >>= 1;
+    a.slots = kMgPartFloats / (a.col_warps * a.nv * 16 * R);
+    const long long groups = (a.M + 15) / 16;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(groups < dev.sm_count ? groups : dev.sm_count));
+    cfg.blockDim = dim3(kMgThreads);
+    cfg.dynamicSmemBytes = mg_smem_bytes<P>(a.chunk_blocks, a.nv);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
+}
+
+template <int VT, int P>
+static int mx_gemv_rows(const MxGemvArgs& a, const DeviceInfo& dev, cudaStream_t s) {
+    if constexpr (P == 1)   // two groups at once need the registers of one column pair
+        if ((a.M + 15) / 16 > dev.sm_count) return mx_gemv_launch<VT, P, 2>(a, dev, s);
+    return mx_gemv_launch<VT, P, 1>(a, dev, s);
+}
+
+template <int VT>
+static int mx_gemv(MxGemvArgs a, int batch, const DeviceInfo& dev, cudaStream_t s) {
+    constexpr int kParts = VT == kSrcF32 ? 2 : 1;
+    const int most = 8 / kParts;
+    const long long v_bytes = VT == kSrcMxfp4 ? 16ll * a.blocks : a.N * (VT == kSrcF32 ? 4 : 2);
+    for (int b = 0; b < batch; b += most) {
+        a.nv = batch - b < most ? batch - b : most;
+        const int cols = a.nv * kParts;
+        const int st = cols <= 2   ? mx_gemv_rows<VT, 1>(a, dev, s)
+                       : cols <= 4 ? mx_gemv_rows<VT, 2>(a, dev, s)
+                                   : mx_gemv_rows<VT, 4>(a, dev, s);
+        if (st != FEATHER_OK) return st;
+        a.v = reinterpret_cast<const unsigned char*>(a.v) + most * v_bytes;
+        if (VT == kSrcMxfp4) a.v_scales += (long long)most * a.blocks;
+        a.out += most * a.M;
+    }
+    return FEATHER_OK;
+}
+
+template <int NT, int CHAINS, int OUT>
+static int mx_gemm_launch(const unsigned char* m_codes, const unsigned char* x_codes, MxGemmArgs a, const DeviceInfo& dev,
+                          cudaStream_t s) {
+    typedef GmLayout<NT, CHAINS> L;
+    auto kernel = mx_gemm_kernel<NT, CHAINS, OUT>;
+    static std::atomic<unsigned long long> configured{0};
+    if (int st = ensure_smem(kernel, L::kBytes, configured)) return st;
+    if (int st = status_word(&a.status)) return st;
+    CUtensorMap map_m, map_x;
+    if (!atc_make_map(&map_m, m_codes, a.blocks * 16, a.M, kGmBox, kGmRows, true) ||
+        !atc_make_map(&map_x, x_codes, a.blocks * 16, a.batch, kGmBox, NT, true))
+        return FEATHER_ERR_LAUNCH;
+    a.tiles_m = (a.M + kGmRows - 1) / kGmRows;
+    a.tiles_x = (a.batch + NT - 1) / NT;
+    const long long tiles = (long long)a.tiles_m * a.tiles_x;
+    if (tiles > 0x7FFFFFFFll - dev.sm_count) return FEATHER_ERR_TOO_LARGE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles < dev.sm_count ? tiles : dev.sm_count));
+    cfg.blockDim = dim3(kGmThreads);
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, map_m, map_x, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
+}
+
+template <int OUT>
+static int mx_gemm(const unsigned char* m_codes, const unsigned char* x_codes, const MxGemmArgs& a, const DeviceInfo& dev,
+                   cudaStream_t s) {
+    return a.batch <= 32    ? mx_gemm_launch<32, 1, OUT>(m_codes, x_codes, a, dev, s)
+           : a.batch <= 64  ? mx_gemm_launch<64, 1, OUT>(m_codes, x_codes, a, dev, s)
+           : a.batch <= 128 ? mx_gemm_launch<128, 1, OUT>(m_codes, x_codes, a, dev, s)
+                            : mx_gemm_launch<224, 1, OUT>(m_codes, x_codes, a, dev, s);
+}
+
+template <int T, int MODE>
+static int rotary_launch(const RotaryArgs& a, const DeviceInfo& dev, cudaStream_t s) {
+    constexpr int V = T == kSrcF32 ? 4 : 8;
+    const bool wide = aligned(a.x, 16) && aligned(a.out, MODE < 0 ? 16 : V) && (a.rotated / 2) % V == 0 && a.dim % V == 0 &&
+                      a.token_stride % V == 0 && a.head_stride % V == 0;
+    const long long most = 16ll * dev.sm_count;
+    const unsigned grid = (unsigned)(a.tokens < most ? a.tokens : most);
+    if (wide) rotary_kernel<T, MODE, V><<<grid, kRotThreads, 0, s>>>(a);
+    else rotary_kernel<T, MODE, 1><<<grid, kRotThreads, 0, s>>>(a);
+    return launch_status();
+}
+
+template <int T>
+static int rotary_mode(const RotaryArgs& a, int mode, const DeviceInfo& dev, cudaStream_t s) {
+    return mode < 0          ? rotary_launch<T, -1>(a, dev, s)
+           : mode == kE5M2   ? rotary_launch<T, kE5M2>(a, dev, s)
+                             : rotary_launch<T, kE4M3>(a, dev, s);
+}
+
 }  // namespace feather
 
 using namespace feather;
@@ -1421,6 +1577,142 @@ int feather_dot_fp8_static(const uint32_t* a, const uint32_t* b, float* out, int
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return mode == FEATHER_MODE_E5M2 ? dot_static_launch<kE5M2>(a, b, out, n_words, *dev, s)
                                      : dot_static_launch<kE4M3>(a, b, out, n_words, *dev, s);
+}
+
+int feather_encode_mxfp4(const void* src, int src_dtype, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols,
+                         void* stream) {
+    if (rows < 0 || cols < 0) return FEATHER_ERR_BAD_ARG;
+    if (src_dtype < 0 || src_dtype > FEATHER_SRC_BF16) return FEATHER_ERR_MODE;
+    if (rows == 0 || cols == 0) return FEATHER_OK;
+    if (!src || !codes || !scales) return FEATHER_ERR_BAD_ARG;
+    if (cols > kMxMaxCols || rows > kMxMaxRows) return FEATHER_ERR_TOO_LARGE;
+    if (!aligned(src, src_dtype == FEATHER_SRC_F32 ? 4 : 2) || !aligned(codes, 16)) return FEATHER_ERR_MISALIGNED;
+    const DeviceInfo* dev = nullptr;
+    if (int st = device_info(&dev)) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return src_dtype == FEATHER_SRC_F16   ? mx_encode_launch<kSrcF16>(src, codes, scales, rows, cols, *dev, s)
+           : src_dtype == FEATHER_SRC_F32 ? mx_encode_launch<kSrcF32>(src, codes, scales, rows, cols, *dev, s)
+                                          : mx_encode_launch<kSrcBF16>(src, codes, scales, rows, cols, *dev, s);
+}
+
+int feather_decode_mxfp4(const uint8_t* codes, const uint8_t* scales, void* dst, int dst_dtype, int64_t rows,
+                         int64_t cols, void* stream) {
+    if (rows < 0 || cols < 0) return FEATHER_ERR_BAD_ARG;
+    if (dst_dtype < 0 || dst_dtype > FEATHER_SRC_BF16) return FEATHER_ERR_MODE;
+    if (rows == 0 || cols == 0) return FEATHER_OK;
+    if (!dst || !codes || !scales) return FEATHER_ERR_BAD_ARG;
+    if (cols > kMxMaxCols || rows > kMxMaxRows) return FEATHER_ERR_TOO_LARGE;
+    if (!aligned(dst, dst_dtype == FEATHER_SRC_F32 ? 4 : 2) || !aligned(codes, 16)) return FEATHER_ERR_MISALIGNED;
+    const DeviceInfo* dev = nullptr;
+    if (int st = device_info(&dev)) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dst_dtype == FEATHER_SRC_F16   ? mx_decode_launch<kSrcF16>(codes, scales, dst, rows, cols, *dev, s)
+           : dst_dtype == FEATHER_SRC_F32 ? mx_decode_launch<kSrcF32>(codes, scales, dst, rows, cols, *dev, s)
+                                          : mx_decode_launch<kSrcBF16>(codes, scales, dst, rows, cols, *dev, s);
+}
+
+int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const void* v, int v_dtype, const uint8_t* v_scales,
+                       float* out, int64_t M, int64_t N, int batch, void* stream) {
+    if (M < 0 || N < 0 || batch < 0) return FEATHER_ERR_BAD_ARG;
+    if (v_dtype < 0 || v_dtype > FEATHER_SRC_MXFP4) return FEATHER_ERR_MODE;
+    if (M == 0 || batch == 0) return FEATHER_OK;
+    if (!out) return FEATHER_ERR_BAD_ARG;
+    if (N > kMxMaxCols || M > kMxMaxRows || batch > 64) return FEATHER_ERR_TOO_LARGE;
+    if (!aligned(out, 4)) return FEATHER_ERR_MISALIGNED;
+    const bool packed = v_dtype == FEATHER_SRC_MXFP4;
+    if (N > 0) {
+        if (!m_codes || !m_scales || !v || (packed && !v_scales)) return FEATHER_ERR_BAD_ARG;
+        if (!aligned(m_codes, 16) || !aligned(v, packed ? 16 : v_dtype == FEATHER_SRC_F32 ? 4 : 2)) return FEATHER_ERR_MISALIGNED;
+    }
+    const DeviceInfo* dev = nullptr;
+    if (int st = device_info(&dev)) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (N == 0)
+        return cudaMemsetAsync(out, 0, (size_t)M * batch * sizeof(float), s) == cudaSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
+    MxGemvArgs a = {};
+    a.codes = m_codes;
+    a.scales = m_scales;
+    a.v = v;
+    a.v_scales = v_scales;
+    a.out = out;
+    a.M = M;
+    a.N = N;
+    a.blocks = mx_blocks(N);
+    switch (v_dtype) {
+        case FEATHER_SRC_F16: return mx_gemv<kSrcF16>(a, batch, *dev, s);
+        case FEATHER_SRC_F32: return mx_gemv<kSrcF32>(a, batch, *dev, s);
+        case FEATHER_SRC_BF16: return mx_gemv<kSrcBF16>(a, batch, *dev, s);
+        default: return mx_gemv<kSrcMxfp4>(a, batch, *dev, s);
+    }
+}
+
+int feather_gemm_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const uint8_t* x_codes, const uint8_t* x_scales,
+                       void* out, int out_dtype, int64_t M, int64_t N, int64_t batch, void* stream) {
+    if (M < 0 || N < 0 || batch < 0) return FEATHER_ERR_BAD_ARG;
+    if (out_dtype < 0 || out_dtype > FEATHER_SRC_BF16) return FEATHER_ERR_MODE;
+    if (M == 0 || batch == 0) return FEATHER_OK;
+    if (!out) return FEATHER_ERR_BAD_ARG;
+    if (N > kMxMaxCols || M > kMxMaxRows - 128 || batch > kMxMaxRows - 256) return FEATHER_ERR_TOO_LARGE;
+    const int size = out_dtype == FEATHER_SRC_F32 ? 4 : 2;
+    if (!aligned(out, size)) return FEATHER_ERR_MISALIGNED;
+    if (N > 0) {
+        if (!m_codes || !m_scales || !x_codes || !x_scales) return FEATHER_ERR_BAD_ARG;
+        if (!aligned(m_codes, 16) || !aligned(x_codes, 16)) return FEATHER_ERR_MISALIGNED;
+    }
+    const DeviceInfo* dev = nullptr;
+    if (int st = device_info(&dev)) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (N == 0)
+        return cudaMemsetAsync(out, 0, (size_t)M * batch * size, s) == cudaSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
+    MxGemmArgs a = {};
+    a.m_scales = m_scales;
+    a.x_scales = x_scales;
+    a.out = out;
+    a.M = (int)M;
+    a.batch = (int)batch;
+    a.blocks = mx_blocks(N);
+    a.align = a.blocks % 8 == 0 && aligned(m_scales, 8) && aligned(x_scales, 8)   ? 8
+              : a.blocks % 4 == 0 && aligned(m_scales, 4) && aligned(x_scales, 4) ? 4
+                                                                                  : 1;
+    return out_dtype == FEATHER_SRC_F16   ? mx_gemm<kSrcF16>(m_codes, x_codes, a, *dev, s)
+           : out_dtype == FEATHER_SRC_F32 ? mx_gemm<kSrcF32>(m_codes, x_codes, a, *dev, s)
+                                          : mx_gemm<kSrcBF16>(m_codes, x_codes, a, *dev, s);
+}
+
+int feather_rotary(const void* x, int dtype, int64_t token_stride, int64_t head_stride, const void* positions,
+                   int wide_positions, const double* inv_freq, void* out, int out_mode, int64_t tokens, int heads, int dim,
+                   int rotated, int layout, float scale, void* stream) {
+    if (tokens < 0 || heads < 0 || dim < 0 || rotated < 2 || rotated % 2 || rotated > dim) return FEATHER_ERR_BAD_ARG;
+    if (dtype < 0 || dtype > FEATHER_SRC_BF16 || out_mode < -1 || out_mode > FEATHER_MODE_E4M3 || layout < 0 || layout > 1)
+        return FEATHER_ERR_MODE;
+    if (out_mode >= 0 && dim % 4) return FEATHER_ERR_BAD_ARG;   // heads are whole packed words
+    if (tokens == 0 || heads == 0) return FEATHER_OK;
+    if (!x || !positions || !inv_freq || !out) return FEATHER_ERR_BAD_ARG;
+    if (rotated > 2 * kRotMaxPairs || (int64_t)heads * dim > (1 << 30)) return FEATHER_ERR_TOO_LARGE;
+    const int size = dtype == FEATHER_SRC_F32 ? 4 : 2;
+    if (!aligned(x, size) || !aligned(out, out_mode < 0 ? size : 4) || !aligned(positions, wide_positions ? 8 : 4) ||
+        !aligned(inv_freq, 8))
+        return FEATHER_ERR_MISALIGNED;
+    const DeviceInfo* dev = nullptr;
+    if (int st = device_info(&dev)) return st;
+    RotaryArgs a = {};
+    a.x = x;
+    a.positions = positions;
+    a.inv_freq = inv_freq;
+    a.out = out;
+    a.tokens = tokens;
+    a.token_stride = token_stride;
+    a.head_stride = head_stride;
+    a.heads = heads;
+    a.dim = dim;
+    a.rotated = rotated;
+    a.wide_positions = wide_positions != 0;
+    a.interleaved = layout == FEATHER_ROTARY_INTERLEAVED;
+    a.scale = scale;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == FEATHER_SRC_F16   ? rotary_mode<kSrcF16>(a, out_mode, *dev, s)
+           : dtype == FEATHER_SRC_F32 ? rotary_mode<kSrcF32>(a, out_mode, *dev, s)
+                                      : rotary_mode<kSrcBF16>(a, out_mode, *dev, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,113 @@
+"""Microscaled 4-bit packers: 32 consecutive elements of the last dimension share a
+power-of-two scale, each element is an E2M1 code (0, .5, 1, 1.5, 2, 3, 4, 6 and
+their negatives).  No counterpart in the reference, whose packers stop at 8 bits
+(feather/packers/fp8.py).
+
+A row of ``n`` elements is ``ceil(n / 32)`` blocks: 16 bytes of codes (the even
+element in the low half of its byte; a short last block is filled up with zero
+codes) and one scale byte ``2 ** (byte - 127)`` each, 255 standing for NaN.  This is
+the layout of the OCP microscaling formats.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from .fp8 import _require_cuda
+
+__all__ = ["pack_mxfp4_tensor", "unpack_mxfp4_tensor"]
+
+BLOCK = 32
+BLOCK_BYTES = 16
+DTYPE_IDS = {torch.float16: _lib.SRC_F16, torch.float32: _lib.SRC_F32, torch.bfloat16: _lib.SRC_BF16}
+_CODE_DTYPES = tuple(d for d in (torch.uint8, getattr(torch, "float4_e2m1fn_x2", None)) if d is not None)
+_SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def blocks_of(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def dtype_id(dtype: torch.dtype, name: str) -> int:
+    if dtype not in DTYPE_IDS:
+        raise TypeError(f"{name} must be float16, bfloat16 or float32, got {dtype}")
+    return DTYPE_IDS[dtype]
+
+
+def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name: str):
+    """Validate a packed operand of ``rows`` rows of ``n`` elements: CUDA, contiguous, bytes,
+    one device, long enough, codes 16-byte aligned."""
+    for t, kind, dtypes in ((codes, "codes", _CODE_DTYPES), (scales, "scales", _SCALE_DTYPES)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}_{kind} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{name}_{kind} must be a CUDA tensor: feather_b200 has no CPU path")
+        if t.dtype not in dtypes:
+            raise ValueError(f"{name}_{kind} must hold packed bytes (uint8), got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}_{kind} must be contiguous")
+    if codes.device != scales.device:
+        raise ValueError(f"{name}_codes and {name}_scales must be on the same device")
+    blocks = blocks_of(n)
+    if codes.numel() < rows * blocks * BLOCK_BYTES:
+        raise ValueError(f"{name}_codes holds {codes.numel()} bytes, {rows}x{n} needs {rows * blocks * BLOCK_BYTES}")
+    if scales.numel() < rows * blocks:
+        raise ValueError(f"{name}_scales holds {scales.numel()} bytes, {rows}x{n} needs {rows * blocks}")
+    if rows * blocks and codes.data_ptr() % 16:
+        raise ValueError(f"{name}_codes must be 16-byte aligned")
+
+
+def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Quantise a float16/bfloat16/float32 tensor of shape ``(..., n)`` along its last dimension.
+
+    Returns ``(codes, scales)``, uint8 of shapes ``(..., 16 * ceil(n / 32))`` and
+    ``(..., ceil(n / 32))``, on ``x``'s device (a CPU tensor is packed on the current CUDA
+    device, as by ``pack_fp8_tensor``).  The scale of a block is ``2 ** (floor(log2 max|x|) - 2)``,
+    codes are rounded to nearest even and saturate at 6 scales; a block with an infinity or a
+    NaN decodes to NaN throughout."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("pack_mxfp4_tensor expects a torch.Tensor")
+    src = dtype_id(x.dtype, "x")
+    if x.dim() == 0:
+        raise ValueError("x needs a last dimension to be packed along")
+    _require_cuda()
+    lib = _lib.load()
+    xd = (x.cuda() if not x.is_cuda else x).contiguous()
+    n = xd.shape[-1]
+    lead, blocks = xd.shape[:-1], blocks_of(n)
+    codes = torch.empty((*lead, blocks * BLOCK_BYTES), dtype=torch.uint8, device=xd.device)
+    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=xd.device)
+    if xd.numel():
+        idx = xd.device.index
+        with torch.cuda.device(idx):
+            _lib.check(lib.feather_encode_mxfp4(xd.data_ptr(), src, codes.data_ptr(), scales.data_ptr(),
+                                                xd.numel() // n, n, _lib.current_stream_ptr(idx)))
+    return (codes, scales) if x.is_cuda else (codes.cpu(), scales.cpu())
+
+
+def unpack_mxfp4_tensor(codes: torch.Tensor, scales: torch.Tensor, n: int | None = None,
+                        dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of packed rows, shape ``(..., n)``; ``n`` defaults to the whole blocks.
+
+    One rounding to ``dtype``: float32 and bfloat16 hold every value (below bfloat16's
+    subnormals aside), float16 rounds and overflows to infinity like any conversion."""
+    dst = dtype_id(dtype, "dtype")
+    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        raise TypeError("codes and scales must be torch.Tensors")
+    if codes.dim() == 0 or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != BLOCK_BYTES * scales.shape[-1]:
+        raise ValueError(f"codes (..., 16 * blocks) and scales (..., blocks) do not match: "
+                         f"{tuple(codes.shape)}, {tuple(scales.shape)}")
+    blocks = scales.shape[-1]
+    n = blocks * BLOCK if n is None else int(n)
+    if blocks_of(n) != blocks or n < 0:
+        raise ValueError(f"n={n} does not have {blocks} blocks of {BLOCK}")
+    lead = codes.shape[:-1]
+    rows = scales[..., 0].numel() if blocks else 0
+    as_packed(codes, scales, rows, n, "m")
+    out = torch.empty((*lead, n), dtype=dtype, device=codes.device)
+    if out.numel():
+        idx = codes.device.index
+        with torch.cuda.device(idx):
+            _lib.check(_lib.load().feather_decode_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows,
+                                                        n, _lib.current_stream_ptr(idx)))
+    return out

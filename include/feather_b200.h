@@ -43,6 +43,10 @@ typedef enum feather_status {
 #define FEATHER_MODE_E4M3 1
 #define FEATHER_SRC_F16 0
 #define FEATHER_SRC_F32 1
+#define FEATHER_SRC_BF16 2      /* the microscaled and rotary entry points only */
+#define FEATHER_SRC_MXFP4 3     /* feather_gemv_mxfp4: a packed vector          */
+#define FEATHER_ROTARY_HALF 0
+#define FEATHER_ROTARY_INTERLEAVED 1
 #define FEATHER_DECODE_KERNEL 0 /* values the GEMV/dot kernels multiply with  */
 #define FEATHER_DECODE_IEEE 1   /* values the reference CPU unpacker returns   */
 
@@ -505,6 +509,71 @@ int64_t feather_dot_workspace_bytes(int64_t n_words);
 int feather_dot_fp8_static(const uint32_t* a, const uint32_t* b, float* out, int64_t n_words,
                            int mode, void* stream);
 int64_t feather_dot_fp8_static_max_words(void);
+
+/*
+ * Microscaled 4-bit floating point (MXFP4): 32 consecutive elements of a row
+ * share a power-of-two scale.  No counterpart in the reference, whose packers
+ * stop at 8 bits.  A row of `cols` elements is ceil(cols / 32) blocks:
+ *   codes    16 bytes per block, two E2M1 codes to a byte, the even element in
+ *            the low half; a short last block is filled up with zero codes.
+ *            16-byte aligned, rows one after the other
+ *   scales   one byte per block, 2^(byte - 127), 255 = NaN; rows one after the
+ *            other, any alignment
+ * Quantising: byte = max(E - 2, 0) with E the FP32 exponent field of the
+ * block's largest magnitude; codes rounded to nearest even, saturating at 6;
+ * a block with an infinity or a NaN gets byte 255 and zero codes.
+ *   src / dst   rows x cols values, contiguous, element aligned; FEATHER_SRC_F16
+ *               / _F32 / _BF16.  Decoding rounds once to the output type (BF16
+ *               and FP32 hold every value exactly down to their subnormals)
+ */
+int feather_encode_mxfp4(const void* src, int src_dtype, uint8_t* codes, uint8_t* scales,
+                         int64_t rows, int64_t cols, void* stream);
+int feather_decode_mxfp4(const uint8_t* codes, const uint8_t* scales, void* dst, int dst_dtype,
+                         int64_t rows, int64_t cols, void* stream);
+
+/*
+ * out[b][r] = sum_j value(m[r][j]) * v[b][j]: a packed MXFP4 matrix times
+ * 0 <= batch <= 64 vectors, FP32 accumulation, eight vectors (four FP32 ones)
+ * per pass over the matrix.  No counterpart in the reference.
+ *   v         batch x N values of v_dtype, contiguous, or FEATHER_SRC_MXFP4:
+ *             packed codes with v_scales (ignored otherwise)
+ *   out       batch x M floats
+ */
+int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const void* v, int v_dtype,
+                       const uint8_t* v_scales, float* out, int64_t M, int64_t N, int batch,
+                       void* stream);
+
+/*
+ * out[b][r] = sum_j value(m[r][j]) * value(x[b][j]), both operands packed
+ * MXFP4, on the tensor cores' microscaled kind; FP32 accumulation, one rounding
+ * to out_dtype (FEATHER_SRC_F16 / _F32 / _BF16).  No counterpart in the reference.
+ *   out       batch x M values
+ */
+int feather_gemm_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const uint8_t* x_codes,
+                       const uint8_t* x_scales, void* out, int out_dtype, int64_t M, int64_t N,
+                       int64_t batch, void* stream);
+
+/*
+ * Rotary positions: the first `rotated` elements of every head are pairs, pair
+ * i of a token at position p turned by p * inv_freq[i] (computed in 64 bits):
+ * (a, b) -> scale * (a cos - b sin, a sin + b cos).  FEATHER_ROTARY_HALF: a =
+ * x[i], b = x[i + rotated / 2]; FEATHER_ROTARY_INTERLEAVED: a = x[2i], b =
+ * x[2i + 1].  The remaining elements pass through.  No counterpart in the
+ * reference.
+ *   x           tokens x heads x dim values of `dtype`, dim contiguous, the other
+ *               strides in elements
+ *   positions   one per token, int64 (wide_positions != 0) or int32
+ *   inv_freq    rotated / 2 doubles; 2 <= rotated <= dim, even, at most 1024
+ *   out         out_mode -1: tokens x heads x dim of `dtype`, contiguous (may be
+ *               x where x is contiguous).  FEATHER_MODE_E5M2 / _E4M3: FP8 codes
+ *               rounded like feather_encode_fp8, heads x tokens x dim bytes,
+ *               dim a multiple of 4 -- a head's codes in one piece, as
+ *               feather_attention_fp8_e5m2 takes them
+ */
+int feather_rotary(const void* x, int dtype, int64_t token_stride, int64_t head_stride,
+                   const void* positions, int wide_positions, const double* inv_freq, void* out,
+                   int out_mode, int64_t tokens, int heads, int dim, int rotated, int layout,
+                   float scale, void* stream);
 
 #ifdef __cplusplus
 }

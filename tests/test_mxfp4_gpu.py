@@ -1,0 +1,387 @@
+"""Microscaled 4-bit operators and rotary positions on the GPU against the 64-bit oracle."""
+import math
+
+import pytest
+import torch
+
+import feather_b200 as fb
+from oracle import mxfp4_oracle as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def values(rows, n, seed, dtype=torch.float32, spread=3.0):
+    """Normal values whose blocks and columns differ in size by powers of two."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, n, generator=gen, device="cuda")
+    return (x * torch.exp2(spread * torch.randn(n, generator=gen, device="cuda")).clamp(2.0 ** -9, 2.0 ** 9)).to(dtype)
+
+
+def packed(rows, n, seed, spread=3.0):
+    return O.quantise(values(rows, n, seed, spread=spread))
+
+
+def same_bits(a, b):
+    return a.shape == b.shape and torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- quantise --
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 32), (3, 31), (2, 33), (5, 64), (1, 2048), (7, 160), (129, 1000), (64, 4096), (1001, 96)])
+def test_pack_is_bit_exact(rows, n, dtype):
+    x = values(rows, n, 11 * rows + n, DTYPES[dtype])
+    codes, scales = fb.pack_mxfp4_tensor(x)
+    want_codes, want_scales = O.quantise(x)
+    assert codes.dtype == scales.dtype == torch.uint8 and codes.device == x.device
+    assert same_bits(scales, want_scales) and same_bits(codes, want_codes)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n", [64, 63])
+def test_pack_edges(dtype, n):
+    t = DTYPES[dtype]
+    info = torch.finfo(t)
+    x = torch.zeros(12, n, dtype=t, device="cuda")
+    x[1] = -0.0
+    x[2, 5] = info.smallest_normal * info.eps      # the type's smallest
+    x[3, :] = info.max
+    x[4, 40] = float("inf")
+    x[5, 2] = float("nan")
+    x[6, 3] = -float("inf")
+    x[7, :8] = torch.tensor([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=t)
+    x[8, :8] = torch.tensor([-4.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0], dtype=t)
+    x[9, 33:37] = torch.tensor([7.9, 6.0, 6.1, -7.9], dtype=t)
+    x[10, 1] = info.tiny
+    x[11, 0], x[11, 1] = info.max, info.tiny       # the far ends in one block
+    codes, scales = fb.pack_mxfp4_tensor(x)
+    want_codes, want_scales = O.quantise(x)
+    assert same_bits(scales, want_scales) and same_bits(codes, want_codes)
+    back = fb.unpack_mxfp4_tensor(codes, scales, n)
+    want = O.dequantise(want_codes, want_scales, n).float()
+    assert torch.equal(back.isnan(), want.isnan()) and torch.equal(back.nan_to_num(7.0), want.nan_to_num(7.0))
+    assert back[4, 32:].isnan().all() and not back[4, :32].isnan().any()
+
+
+def test_pack_shapes_views_and_cpu_input():
+    x = values(6, 64, 5)
+    whole = fb.pack_mxfp4_tensor(x)
+    lead = fb.pack_mxfp4_tensor(x.view(2, 3, 64))
+    assert lead[0].shape == (2, 3, 32) and lead[1].shape == (2, 3, 2)
+    assert same_bits(lead[0].view(6, 32), whole[0]) and same_bits(lead[1].view(6, 2), whole[1])
+    one = fb.pack_mxfp4_tensor(x[2])
+    assert same_bits(one[0], whole[0][2]) and same_bits(one[1], whole[1][2])
+    t = values(64, 6, 6)
+    assert all(same_bits(a, b) for a, b in zip(fb.pack_mxfp4_tensor(t.T), fb.pack_mxfp4_tensor(t.T.contiguous())))
+    odd = torch.empty(1 + 6 * 64, device="cuda")[1:].view(6, 64).copy_(x)       # a start off the 16-byte grid
+    assert odd.data_ptr() % 16 and all(same_bits(a, b) for a, b in zip(fb.pack_mxfp4_tensor(odd), whole))
+    host = fb.pack_mxfp4_tensor(x.cpu())
+    assert not host[0].is_cuda and same_bits(host[0].cuda(), whole[0]) and same_bits(host[1].cuda(), whole[1])
+    for shape in ((0, 64), (3, 0), (0,)):
+        c, s = fb.pack_mxfp4_tensor(torch.empty(shape, device="cuda"))
+        assert c.numel() == 0 and s.numel() == 0
+        assert fb.unpack_mxfp4_tensor(c, s, shape[-1]).shape == shape
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 32), (3, 31), (9, 257), (5, 96), (130, 1024), (2, 5000)])
+def test_unpack_every_byte_and_scale(rows, n, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(rows + n)
+    blocks = -(-n // 32)
+    codes = torch.randint(0, 256, (rows, 16 * blocks), generator=gen, device="cuda").to(torch.uint8)
+    scales = torch.randint(0, 256, (rows, blocks), generator=gen, device="cuda").to(torch.uint8)
+    got = fb.unpack_mxfp4_tensor(codes, scales, n, DTYPES[dtype])
+    # the exact value, once through FP32 (exact but for what overflows there as well) and rounded
+    want = O.dequantise(codes, scales, n).float().to(DTYPES[dtype])
+    assert got.dtype == DTYPES[dtype] and got.shape == (rows, n)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(torch.where(got.isnan(), 0, got), torch.where(want.isnan(), 0, want))
+
+
+# -------------------------------------------------------------------- gemv --
+def gemv_bound(m, v, split):
+    """Per element: a block's 32 products are added by the tensor core, whose FP32 sum may lose 2^-22 of the products' size
+    per instruction (two have products of the block); two scalings round (2^-24 each); a warp adds
+    its blocks, four lanes, at most 16 warps and the chunks in FP32 (2^-24 per addition); an FP32 vector is split with an error of
+    2^-24 per element."""
+    blocks = -(-m.shape[1] // 32)
+    steps = math.ceil(blocks / 4) + 2 + 16 + 2 + (1 if split else 0) + math.ceil(blocks / 192)
+    return (v.abs() @ m.abs().T) * (2 * 2.0 ** -22 + steps * 2.0 ** -24) + 1e-44
+
+
+@pytest.mark.parametrize("vector", ["fp16", "bf16", "fp32", "mxfp4"])
+@pytest.mark.parametrize("M,N,batch", [(1, 1, 1), (1, 32, 1), (17, 33, 1), (16, 128, 2), (3, 4000, 1), (256, 2048, 1), (250, 2080, 3),
+                                       (2400, 256, 1), (2500, 100, 5), (4800, 4096, 1), (40, 30000, 2), (100, 1024, 8), (33, 640, 11)])
+def test_gemv(M, N, batch, vector):
+    codes, scales = packed(M, N, M + N)
+    m = O.dequantise(codes, scales, N)
+    if vector == "mxfp4":
+        v, v_scales = packed(batch, N, 7 * M + N)
+        wide = O.dequantise(v, v_scales, N)
+    else:
+        v, v_scales = values(batch, N, 7 * M + N, DTYPES[vector], spread=2.0), None
+        wide = v.double()
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N), v_scales=v_scales)
+    assert got.dtype == torch.float32 and got.shape == (batch, M)
+    want = wide @ m.T
+    err = (got.double() - want).abs()
+    assert bool((err <= gemv_bound(m, wide, vector == "fp32")).all()), (err / gemv_bound(m, wide, vector == "fp32")).max()
+    one = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v[0], (M, N), v_scales=None if v_scales is None else v_scales[0])
+    assert one.shape == (M,) and torch.equal(one, fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v[:1], (M, N),
+                                             v_scales=None if v_scales is None else v_scales[:1])[0])
+    assert torch.equal(got, fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N), v_scales=v_scales))   # the same bits again
+
+
+def test_gemv_large():
+    M, N = 9000, 16384
+    codes, scales = packed(M, N, 3)
+    m = O.dequantise(codes, scales, N)
+    for dtype in DTYPES:
+        v = values(1, N, 4, DTYPES[dtype], spread=2.0)
+        got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+        assert bool(((got.double() - v.double() @ m.T).abs() <= gemv_bound(m, v.double(), dtype == "fp32")).all())
+
+
+def test_gemv_more_rows_than_partial_sums_fit():
+    # one column tile, so that every warp takes rows; more 16-row groups per CTA than one round of partial sums
+    M, N = 148 * 16 * 2 * 400 + 5, 32
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    codes = torch.randint(0, 256, (M, 16), generator=gen, device="cuda").to(torch.uint8)
+    scales = torch.randint(120, 130, (M, 1), generator=gen, device="cuda").to(torch.uint8)
+    v = values(1, N, 4, torch.bfloat16)
+    m = O.dequantise(codes, scales, N)
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+    assert bool(((got.double() - v.double() @ m.T).abs() <= gemv_bound(m, v.double(), False)).all())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_gemv_values_that_are_not_finite_and_far_scales(dtype):
+    M, N = 40, 256
+    codes, scales = packed(M, N, 1)
+    scales = scales.clone()
+    scales[3, 2] = 255                                # a NaN block: its row only
+    m = O.dequantise(codes, scales, N)
+    v = values(4, N, 2, DTYPES[dtype], spread=1.0)
+    v[1, 70] = float("inf")
+    v[2, 200] = float("nan")
+    v[3] = 0
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N)).double()
+    want = v.double() @ m.T
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[want.isinf()], want[want.isinf()])
+    fine = want.isfinite()
+    bound = gemv_bound(m.nan_to_num(0.0), v.double().nan_to_num(0.0, 0.0, 0.0), dtype == "fp32")
+    assert bool(((got - want).abs()[fine] <= bound[fine]).all())
+    # blocks that differ by 2^40 in both operands, and far from one
+    far = torch.exp2(torch.tensor([-20.0, 20.0, -4.0, 4.0], device="cuda").repeat_interleave(64)) if dtype != "fp16" else \
+        torch.exp2(torch.tensor([-10.0, 10.0, -4.0, 4.0], device="cuda").repeat_interleave(64))
+    v2 = (torch.randn(1, N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * far).to(DTYPES[dtype])
+    codes, scales = O.quantise(values(M, N, 9, spread=0.0) / far.double().flip(0))
+    m = O.dequantise(codes, scales, N)
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v2, (M, N)).double()
+    assert bool(((got - v2.double() @ m.T).abs() <= gemv_bound(m, v2.double(), dtype == "fp32")).all())
+
+
+# -------------------------------------------------------------------- gemm --
+def gemm_bound(m, x, dtype):
+    """Per element: N / 64 products in a row add into one FP32 sum, each may lose 2^-22 of the products' size so far (the
+    tensor core does not round to nearest); one rounding to the output type."""
+    steps = math.ceil(m.shape[1] / 64) + 1
+    size = x.abs() @ m.abs().T
+    return size * steps * 2.0 ** -22 + (x @ m.T).abs() * torch.finfo(dtype).eps / 2 * 1.001 + torch.finfo(dtype).tiny
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("M,N,batch", [(1, 1, 1), (128, 256, 32), (128, 64, 1), (130, 33, 7), (200, 1000, 40), (77, 2080, 64),
+                                       (1000, 288, 100), (300, 5000, 129), (2048, 512, 225), (513, 1536, 449), (5000, 160, 300)])
+def test_gemm(M, N, batch, dtype):
+    codes, scales = packed(M, N, M + N, spread=1.0)
+    x, x_scales = packed(batch, N, 5 * M + N, spread=1.0)
+    got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N), out_dtype=DTYPES[dtype])
+    assert got.dtype == DTYPES[dtype] and got.shape == (batch, M)
+    m, w = O.dequantise(codes, scales, N), O.dequantise(x, x_scales, N)
+    bound = gemm_bound(m, w, DTYPES[dtype])
+    err = (got.double() - w @ m.T).abs()
+    assert bool((err <= bound).all()), (err / bound).max()
+    assert torch.equal(got, fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N), out_dtype=DTYPES[dtype]))
+
+
+def test_gemm_every_place_and_scale_is_its_own():
+    # one element and one scale at a time: a row or a scale in the wrong place shows as a wrong number
+    M, N, batch = 256, 512, 256
+    codes = torch.zeros(M, N // 2, dtype=torch.uint8, device="cuda")
+    x = torch.full((batch, N // 2), 0x22, dtype=torch.uint8, device="cuda")       # ones
+    k = (torch.arange(M, device="cuda") * 37) % N
+    codes[torch.arange(M, device="cuda"), k // 2] = torch.where(k % 2 == 0, 2, 32).to(torch.uint8)   # a one at column k of each row
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    scales = torch.randint(117, 138, (M, N // 32), generator=gen, device="cuda").to(torch.uint8)
+    x_scales = torch.randint(117, 138, (batch, N // 32), generator=gen, device="cuda").to(torch.uint8)
+    got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N))
+    e = scales[torch.arange(M, device="cuda"), k // 32].int()[None, :] + x_scales.int()[:, k // 32]
+    assert torch.equal(got, torch.exp2((e - 254).float()))
+
+
+def test_gemm_nan_scales_stay_in_their_row():
+    M, N, batch = 150, 320, 50
+    codes, scales = packed(M, N, 1, spread=1.0)
+    x, x_scales = packed(batch, N, 2, spread=1.0)
+    scales, x_scales = scales.clone(), x_scales.clone()
+    scales[7, 9], x_scales[31, 0] = 255, 255
+    got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N))
+    want = O.dequantise(x, x_scales, N) @ O.dequantise(codes, scales, N).T
+    assert torch.equal(got.isnan(), want.isnan())
+
+
+# ------------------------------------------------------------------ rotary --
+def rotary_bound(x, positions, inv_freq, layout, scale, dtype):
+    """Angle: |p f| 2^-51 and 2 pi 2^-26; sine and cosine 2^-23; two products and a sum; the output's rounding."""
+    angle = positions.double().abs().max() * inv_freq.max() * 2.0 ** -51 + 2 * math.pi * 2.0 ** -26 + 2.0 ** -23 + 3 * 2.0 ** -24
+    half = inv_freq.numel()
+    size = torch.zeros_like(x, dtype=torch.float64)
+    for i in range(half):
+        a, b = (i, i + half) if layout == "half" else (2 * i, 2 * i + 1)
+        size[..., a] = size[..., b] = scale * (x[..., a].double().abs() + x[..., b].double().abs())
+    return size * angle + O.rotate(x, positions, inv_freq, layout, scale).abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("tokens,heads,dim,rotated,start", [(1, 1, 2, 2, 0), (1, 36, 64, 64, 100003), (5, 3, 80, 40, 7), (3, 2, 96, 34, 2 ** 20),
+                                                            (130, 4, 128, 64, 2 ** 31 - 131), (17, 1, 1024, 1024, 50), (2, 5, 33, 6, 9)])
+def test_rotary(tokens, heads, dim, rotated, start, dtype, layout):
+    gen = torch.Generator(device="cuda").manual_seed(tokens + dim)
+    x = torch.randn(tokens, heads, dim, generator=gen, device="cuda").to(DTYPES[dtype])
+    inv = fb.rotary_frequencies(rotated)
+    for kind in (torch.int64, torch.int32):
+        pos = torch.arange(start, start + tokens, device="cuda").to(kind)
+        got = fb.rotary_gpu(x, pos, inv, layout, scale=1.25)
+        bound = rotary_bound(x, pos, inv, layout, 1.25, DTYPES[dtype])
+        assert got.dtype == x.dtype and bool(((got.double() - O.rotate(x, pos, inv, layout, 1.25)).abs() <= bound).all())
+        assert torch.equal(got[..., rotated:], x[..., rotated:])
+    again = x.clone()
+    assert fb.rotary_gpu(again, pos, inv, layout, scale=1.25, out=again) is again and torch.equal(again, got)
+
+
+@pytest.mark.parametrize("mode,kind,half_step,tiny", [("E5M2", torch.float8_e5m2, 2.0 ** -3, 2.0 ** -17), ("E4M3", torch.float8_e4m3fn, 2.0 ** -4, 2.0 ** -10)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("tokens,heads,dim,rotated,layout", [(1, 4, 64, 64, "half"), (33, 3, 128, 64, "interleaved"), (7, 2, 20, 6, "half")])
+def test_rotary_packed(tokens, heads, dim, rotated, layout, dtype, mode, kind, half_step, tiny):
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn(tokens, heads, dim, generator=gen, device="cuda").to(DTYPES[dtype])
+    pos, inv = torch.randint(0, 5000, (tokens,), generator=gen, device="cuda"), fb.rotary_frequencies(rotated)
+    words = fb.rotary_gpu(x, pos, inv, layout, mode=mode)
+    assert words.dtype == torch.uint32 and words.shape == (heads, tokens, dim // 4) and words.feather_mode == mode
+    got = words.as_subclass(torch.Tensor).view(kind).double().transpose(0, 1)
+    want = O.rotate(x, pos, inv, layout)
+    slack = rotary_bound(x, pos, inv, layout, 1.0, torch.float32)
+    assert bool(((got - want).abs() <= want.abs() * half_step + tiny + 2 * slack).all())
+    # away from the borders the words are the packer's of the same values
+    dense = fb.rotary_gpu(x.float(), pos, inv, layout).transpose(0, 1).contiguous()
+    assert torch.equal(words.as_subclass(torch.Tensor).flatten().view(torch.int32), fb.pack_fp8_tensor(dense, mode).as_subclass(torch.Tensor).view(torch.int32))
+
+
+def test_rotary_strides_and_padding_rows_left_alone():
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn(9, 3, 4, 64, generator=gen, device="cuda", dtype=torch.float16)
+    inv, pos = fb.rotary_frequencies(64), torch.arange(9, device="cuda")
+    k = qkv[:, 1]                                             # a slice of a fused projection: strided tokens
+    assert not k.is_contiguous() and torch.equal(fb.rotary_gpu(k, pos, inv), fb.rotary_gpu(k.contiguous(), pos, inv))
+    heads_first = qkv[:, 0].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(fb.rotary_gpu(heads_first, pos, inv), fb.rotary_gpu(qkv[:, 0].contiguous(), pos, inv))
+    odd = torch.empty(1 + 9 * 4 * 64, device="cuda", dtype=torch.float16)[1:].view(9, 4, 64).copy_(k)
+    assert torch.equal(fb.rotary_gpu(odd, pos, inv), fb.rotary_gpu(k, pos, inv))
+    out = torch.full((10, 4, 64), 7.0, device="cuda", dtype=torch.float16)
+    fb.rotary_gpu(k, pos, inv, out=out[:9])
+    assert bool((out[9] == 7.0).all())
+    assert fb.rotary_gpu(qkv[:0, 0], pos[:0], inv).shape == (0, 4, 64)
+
+
+# ---------------------------------------------------------------- together --
+def test_projections_rotation_and_attention_together():
+    """Weights packed to 4 bits, a prompt projected, queries and keys rotated and packed, attended, packed again and
+    projected back: each step against the oracle on the step's own inputs, and one token's GEMV against the prompt's GEMM."""
+    hidden, heads, dim, tokens = 512, 4, 64, 96
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    w = [fb.pack_mxfp4_tensor(0.05 * torch.randn(heads * dim, hidden, generator=gen, device="cuda")) for _ in range(3)]
+    wo = fb.pack_mxfp4_tensor(0.05 * torch.randn(hidden, heads * dim, generator=gen, device="cuda"))
+    x = torch.randn(tokens, hidden, generator=gen, device="cuda").to(torch.bfloat16)
+    xc, xs = fb.pack_mxfp4_tensor(x)
+    q, k, v = (fb.gemm_mxfp4_acc_fp32_gpu(*m, xc, xs, (heads * dim, hidden)) for m in w)
+    for m, y in zip(w, (q, k, v)):
+        m64, x64 = O.dequantise(*m, hidden), O.dequantise(xc, xs, hidden)
+        assert bool(((y.double() - x64 @ m64.T).abs() <= gemm_bound(m64, x64, torch.float32)).all())
+        one = fb.gemv_mxfp4_acc_fp32_gpu(*m, xc[5], (heads * dim, hidden), v_scales=xs[5])
+        size = (x64[5:6].abs() @ m64.abs().T)[0]
+        assert bool(((one - y[5]).abs() <= size * 2.0 ** -18).all())
+    inv, pos = fb.rotary_frequencies(dim), torch.arange(1000, 1000 + tokens, device="cuda")
+    qp, kp = (fb.rotary_gpu(t.view(tokens, heads, dim), pos, inv, mode="E5M2") for t in (q, k))
+    outs = []
+    from feather_b200.routines.attention import flash_attention_fp8_e5m2_acc_fp32_gpu
+    for h in range(heads):
+        vh = fb.pack_fp8_tensor(v.view(tokens, heads, dim)[:, h].contiguous(), "E5M2")
+        o = flash_attention_fp8_e5m2_acc_fp32_gpu(qp[h], kp[h], vh, tokens, dim // 4)
+        f = [fb.unpack_fp8_tensor(t.contiguous(), "E5M2").view(tokens, dim).double() for t in (qp[h], kp[h], vh)]
+        s = torch.zeros(tokens, 128, dtype=torch.float64, device="cuda")      # the last key tile is filled with zero scores
+        s[:, :tokens] = f[0] @ f[1].T / dim ** 0.5
+        want = torch.softmax(s, -1)[:, :tokens] @ f[2]
+        assert bool(((o.double() - want).abs() <= 5e-4 * f[2].abs().max()).all())
+        outs.append(o)
+    oc, os_ = fb.pack_mxfp4_tensor(torch.cat(outs, -1))
+    y = fb.gemm_mxfp4_acc_fp32_gpu(*wo, oc, os_, (hidden, heads * dim), out_dtype=torch.bfloat16)
+    m64, x64 = O.dequantise(*wo, heads * dim), O.dequantise(oc, os_, heads * dim)
+    assert bool(((y.double() - x64 @ m64.T).abs() <= gemm_bound(m64, x64, torch.bfloat16)).all())
+
+
+def test_captured_and_replayed_on_another_stream():
+    M, N = 300, 512
+    w = packed(M, N, 1)
+    x = torch.randn(4, N, device="cuda")
+    inv, pos = fb.rotary_frequencies(60), torch.arange(4, device="cuda")
+    stream = torch.cuda.Stream()
+
+    def chain():
+        c, s = fb.pack_mxfp4_tensor(x)
+        a = fb.gemm_mxfp4_acc_fp32_gpu(*w, c, s, (M, N))
+        b = fb.gemv_mxfp4_acc_fp32_gpu(*w, x, (M, N))
+        r = fb.rotary_gpu(a.view(4, 5, 60), pos, inv)
+        return c, s, a, b, r, fb.unpack_mxfp4_tensor(c, s)
+    with torch.cuda.stream(stream):
+        chain()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = chain()
+    for seed in (1, 2):
+        x.copy_(torch.randn(4, N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)))
+        pos += 3
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, chain()))
+
+
+def test_refusals_on_the_gpu():
+    codes, scales = packed(8, 64, 1)
+    x = torch.randn(64, device="cuda")
+    ok = dict(m_codes=codes, m_scales=scales, v=x, m_shape=(8, 64))
+    fb.gemv_mxfp4_acc_fp32_gpu(**ok)
+    for bad in (dict(v=x[:63]), dict(v=torch.randn(1, 2, 64, device="cuda")), dict(v=torch.randn(128, device="cuda")[::2]),
+                dict(m_shape=(9, 64)), dict(m_shape=(8, 65)), dict(m_scales=scales[:4]), dict(m_codes=codes[:, ::2]),
+                dict(out=torch.empty(9, device="cuda")), dict(out=torch.empty(8, device="cuda", dtype=torch.float16)),
+                dict(v=torch.randn(65, 64, device="cuda")), dict(v_scales=scales[0]),
+                dict(m_codes=torch.zeros(8 * 32 + 8, dtype=torch.uint8, device="cuda")[8:].view(8, 32))):
+        with pytest.raises(ValueError):
+            fb.gemv_mxfp4_acc_fp32_gpu(**{**ok, **bad})
+    with pytest.raises(TypeError):
+        fb.gemv_mxfp4_acc_fp32_gpu(**{**ok, "v": x.double()})
+    with pytest.raises(ValueError):
+        fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, codes[:, :16].contiguous(), scales, (8, 64))
+    with pytest.raises(ValueError):
+        fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, codes, scales[:7], (8, 64))
+    h, inv, pos = torch.randn(4, 2, 64, device="cuda"), fb.rotary_frequencies(64), torch.arange(4, device="cuda")
+    for bad in (dict(x=h[0]), dict(positions=pos[:3]), dict(positions=pos.float()), dict(inv_freq=inv.float()), dict(inv_freq=inv.repeat(2)),
+                dict(inv_freq=inv[:0]), dict(x=h.transpose(1, 2)), dict(out=torch.empty(4, 2, 64, device="cuda", dtype=torch.float16)),
+                dict(x=h[..., :62], inv_freq=inv[:31], mode="E5M2")):
+        with pytest.raises(ValueError):
+            fb.rotary_gpu(**{**dict(x=h, positions=pos, inv_freq=inv), **bad})
+    assert bool((fb.gemv_mxfp4_acc_fp32_gpu(codes[:, :0].contiguous(), scales[:, :0].contiguous(), x[:0], (8, 0)) == 0).all())
+    assert fb.gemv_mxfp4_acc_fp32_gpu(codes[:0], scales[:0], x, (0, 64)).shape == (0,)
+    assert fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, codes[:0], scales[:0], (8, 64)).shape == (0, 8)
