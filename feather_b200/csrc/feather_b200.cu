@@ -961,6 +961,11 @@ static int mx_gemm_launch(const unsigned char* m_codes, const unsigned char* x_c
     if (!atc_make_map(&map_m, m_codes, a.blocks * 16, a.M, kGmBox, kGmRows, true) ||
         !atc_make_map(&map_x, x_codes, a.blocks * 16, a.batch, kGmBox, NT, true))
         return FEATHER_ERR_LAUNCH;
+    constexpr int kSize = OUT == kSrcF32 ? 4 : 2;
+    CUtensorMap map_out = {};
+    a.bulk = (long long)a.M * kSize % 16 == 0 && aligned(a.out, 16);
+    if (a.bulk && !gm_make_out_map(&map_out, a.out, kSize, OUT == kSrcBF16, a.M, a.batch, kGmPiece / (32 * kSize)))
+        return FEATHER_ERR_LAUNCH;
     a.tiles_m = (a.M + kGmRows - 1) / kGmRows;
     a.tiles_x = (a.batch + NT - 1) / NT;
     const long long tiles = (long long)a.tiles_m * a.tiles_x;
@@ -975,7 +980,7 @@ static int mx_gemm_launch(const unsigned char* m_codes, const unsigned char* x_c
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, map_m, map_x, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, map_m, map_x, map_out, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
 }
 
 template <int OUT>
@@ -1671,9 +1676,9 @@ int feather_gemm_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const ui
     a.M = (int)M;
     a.batch = (int)batch;
     a.blocks = mx_blocks(N);
-    a.align = a.blocks % 8 == 0 && aligned(m_scales, 8) && aligned(x_scales, 8)   ? 8
+    a.align = a.blocks % 16 == 0 && aligned(m_scales, 16) && aligned(x_scales, 16) ? 16
               : a.blocks % 4 == 0 && aligned(m_scales, 4) && aligned(x_scales, 4) ? 4
-                                                                                  : 1;
+                                                                                   : 1;
     return out_dtype == FEATHER_SRC_F16   ? mx_gemm<kSrcF16>(m_codes, x_codes, a, *dev, s)
            : out_dtype == FEATHER_SRC_F32 ? mx_gemm<kSrcF32>(m_codes, x_codes, a, *dev, s)
                                           : mx_gemm<kSrcBF16>(m_codes, x_codes, a, *dev, s);

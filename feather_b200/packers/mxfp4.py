@@ -34,10 +34,19 @@ def dtype_id(dtype: torch.dtype, name: str) -> int:
     return DTYPE_IDS[dtype]
 
 
-def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name: str):
-    """Validate a packed operand of ``rows`` rows of ``n`` elements: CUDA, contiguous, bytes,
-    one device, long enough, codes 16-byte aligned."""
-    for t, kind, dtypes in ((codes, "codes", _CODE_DTYPES), (scales, "scales", _SCALE_DTYPES)):
+def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name: str) -> int:
+    """Validate a packed operand of ``rows`` rows of ``n`` elements -- CUDA, contiguous, bytes,
+    one device, long enough -- and return its device's index.  (The library checks that codes
+    are 16-byte aligned.)"""
+    blocks = (n + BLOCK - 1) // BLOCK
+    if (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.is_cuda and scales.is_cuda
+            and codes.dtype in _CODE_DTYPES and scales.dtype in _SCALE_DTYPES and codes.is_contiguous()
+            and scales.is_contiguous() and codes.numel() >= rows * blocks * BLOCK_BYTES and scales.numel() >= rows * blocks):
+        idx = codes.get_device()
+        if idx == scales.get_device():
+            return idx
+    for t, kind, dtypes, need in ((codes, "codes", _CODE_DTYPES, rows * blocks * BLOCK_BYTES),
+                                  (scales, "scales", _SCALE_DTYPES, rows * blocks)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}_{kind} must be a torch.Tensor")
         if not t.is_cuda:
@@ -46,15 +55,18 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
             raise ValueError(f"{name}_{kind} must hold packed bytes (uint8), got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name}_{kind} must be contiguous")
-    if codes.device != scales.device:
-        raise ValueError(f"{name}_codes and {name}_scales must be on the same device")
-    blocks = blocks_of(n)
-    if codes.numel() < rows * blocks * BLOCK_BYTES:
-        raise ValueError(f"{name}_codes holds {codes.numel()} bytes, {rows}x{n} needs {rows * blocks * BLOCK_BYTES}")
-    if scales.numel() < rows * blocks:
-        raise ValueError(f"{name}_scales holds {scales.numel()} bytes, {rows}x{n} needs {rows * blocks}")
-    if rows * blocks and codes.data_ptr() % 16:
-        raise ValueError(f"{name}_codes must be 16-byte aligned")
+        if t.numel() < need:
+            raise ValueError(f"{name}_{kind} holds {t.numel()} bytes, {rows}x{n} needs {need}")
+    raise ValueError(f"{name}_codes and {name}_scales must be on the same device")
+
+
+def call(fn, idx: int, args) -> None:
+    """``fn(*args, stream)`` with device ``idx`` current, on its current stream."""
+    if torch._C._cuda_getDevice() == idx:
+        _lib.check(fn(*args, _lib.current_stream_ptr(idx)))
+    else:
+        with torch.cuda.device(idx):
+            _lib.check(fn(*args, _lib.current_stream_ptr(idx)))
 
 
 def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -70,19 +82,21 @@ def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     src = dtype_id(x.dtype, "x")
     if x.dim() == 0:
         raise ValueError("x needs a last dimension to be packed along")
-    _require_cuda()
+    if not x.is_cuda:
+        _require_cuda()
+        codes, scales = pack_mxfp4_tensor(x.cuda())
+        return codes.cpu(), scales.cpu()
     lib = _lib.load()
-    xd = (x.cuda() if not x.is_cuda else x).contiguous()
-    n = xd.shape[-1]
-    lead, blocks = xd.shape[:-1], blocks_of(n)
-    codes = torch.empty((*lead, blocks * BLOCK_BYTES), dtype=torch.uint8, device=xd.device)
-    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=xd.device)
-    if xd.numel():
-        idx = xd.device.index
-        with torch.cuda.device(idx):
-            _lib.check(lib.feather_encode_mxfp4(xd.data_ptr(), src, codes.data_ptr(), scales.data_ptr(),
-                                                xd.numel() // n, n, _lib.current_stream_ptr(idx)))
-    return (codes, scales) if x.is_cuda else (codes.cpu(), scales.cpu())
+    x = x.contiguous()
+    *lead, n = x.shape
+    blocks = (n + BLOCK - 1) // BLOCK
+    device = x.device
+    codes = torch.empty(*lead, blocks * BLOCK_BYTES, dtype=torch.uint8, device=device)
+    scales = torch.empty(*lead, blocks, dtype=torch.uint8, device=device)
+    total = x.numel()
+    if total:
+        call(lib.feather_encode_mxfp4, device.index, (x.data_ptr(), src, codes.data_ptr(), scales.data_ptr(), total // n, n))
+    return codes, scales
 
 
 def unpack_mxfp4_tensor(codes: torch.Tensor, scales: torch.Tensor, n: int | None = None,
@@ -101,13 +115,9 @@ def unpack_mxfp4_tensor(codes: torch.Tensor, scales: torch.Tensor, n: int | None
     n = blocks * BLOCK if n is None else int(n)
     if blocks_of(n) != blocks or n < 0:
         raise ValueError(f"n={n} does not have {blocks} blocks of {BLOCK}")
-    lead = codes.shape[:-1]
-    rows = scales[..., 0].numel() if blocks else 0
-    as_packed(codes, scales, rows, n, "m")
-    out = torch.empty((*lead, n), dtype=dtype, device=codes.device)
-    if out.numel():
-        idx = codes.device.index
-        with torch.cuda.device(idx):
-            _lib.check(_lib.load().feather_decode_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows,
-                                                        n, _lib.current_stream_ptr(idx)))
+    rows = scales.numel() // blocks if blocks else 0
+    idx = as_packed(codes, scales, rows, n, "m")
+    out = torch.empty(*codes.shape[:-1], n, dtype=dtype, device=codes.device)
+    if rows:
+        call(_lib.load().feather_decode_mxfp4, idx, (codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows, n))
     return out

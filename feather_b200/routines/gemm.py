@@ -7,10 +7,12 @@ multiplies packed FP8 (feather/routines/gemv.py).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import _lib
-from ..packers.mxfp4 import BLOCK_BYTES, as_packed, blocks_of, dtype_id
+from ..packers.mxfp4 import BLOCK_BYTES, as_packed, blocks_of, call, dtype_id
 
 __all__ = ["gemv_mxfp4_acc_fp32_gpu", "gemm_mxfp4_acc_fp32_gpu"]
 
@@ -26,15 +28,9 @@ def _shape(m_shape) -> tuple[int, int]:
     return M, N
 
 
-def _result(out, shape, dtype, device):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    n = 1
-    for s in shape:
-        n *= s
-    if (out.dtype != dtype or out.numel() != n or out.device != device or not out.is_contiguous()):
+def _check_out(out, n, dtype, device):
+    if out.dtype != dtype or out.numel() != n or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {dtype} tensor of {n} elements on the operands' device")
-    return out
 
 
 def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: torch.Tensor, m_shape,
@@ -47,41 +43,41 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
     packed codes together with ``v_scales``.  Eight vectors (four float32 ones) go through one
     pass over the matrix; at most 64."""
     M, N = _shape(m_shape)
-    as_packed(m_codes, m_scales, M, N, "m")
+    idx = as_packed(m_codes, m_scales, M, N, "m")
     if not isinstance(v, torch.Tensor):
         raise TypeError("v must be a torch.Tensor")
-    if v.dim() not in (1, 2):
+    dims = v.dim()
+    if dims != 1 and dims != 2:
         raise ValueError("v must be one vector or a (batch, N) tensor of them")
-    batch = 1 if v.dim() == 1 else v.shape[0]
+    shape = v.shape
+    batch = 1 if dims == 1 else shape[0]
     if v_scales is None:
         if not v.is_cuda:
             raise ValueError("v must be a CUDA tensor: feather_b200 has no CPU path")
         v_dtype = dtype_id(v.dtype, "v (without v_scales)")
-        if v.shape[-1] != N:
-            raise ValueError(f"v has {v.shape[-1]} elements per vector, the matrix has N={N}")
+        if shape[-1] != N:
+            raise ValueError(f"v has {shape[-1]} elements per vector, the matrix has N={N}")
         if not v.is_contiguous():
             raise ValueError("v must be contiguous")
         scales_ptr = None
     else:
         as_packed(v, v_scales, batch, N, "v")
-        if v.shape[-1] != blocks_of(N) * BLOCK_BYTES:
-            raise ValueError(f"packed vectors of N={N} have {blocks_of(N) * BLOCK_BYTES} bytes each, got {v.shape[-1]}")
+        if shape[-1] != blocks_of(N) * BLOCK_BYTES:
+            raise ValueError(f"packed vectors of N={N} have {blocks_of(N) * BLOCK_BYTES} bytes each, got {shape[-1]}")
         v_dtype, scales_ptr = _lib.SRC_MXFP4, v_scales.data_ptr()
-    if v.device != m_codes.device:
+    if v.get_device() != idx:
         raise ValueError("m and v must be on the same device")
     if batch > MAX_VECTORS:
         raise ValueError(f"at most {MAX_VECTORS} vectors: pack them and use gemm_mxfp4_acc_fp32_gpu")
-    out = _result(out, (M,) if v.dim() == 1 else (batch, M), torch.float32, m_codes.device)
+    if out is not None:
+        _check_out(out, batch * M, torch.float32, v.device)
+    elif dims == 1:
+        out = torch.empty(M, dtype=torch.float32, device=v.device)
+    else:
+        out = torch.empty(batch, M, dtype=torch.float32, device=v.device)
     if M and batch:
-        idx = m_codes.device.index
-        fn = _lib.load().feather_gemv_mxfp4
-        args = (m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr, out.data_ptr(), M, N, batch,
-                _lib.current_stream_ptr(idx))
-        if torch.cuda.current_device() == idx:
-            _lib.check(fn(*args))
-        else:
-            with torch.cuda.device(idx):
-                _lib.check(fn(*args))
+        call(_lib.load().feather_gemv_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype,
+                                                   scales_ptr, out.data_ptr(), M, N, batch))
     return out
 
 
@@ -96,26 +92,20 @@ def gemm_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, x_cod
     ``(..., N)``: the leading dimensions are rows)."""
     M, N = _shape(m_shape)
     dst = dtype_id(out_dtype, "out_dtype")
-    as_packed(m_codes, m_scales, M, N, "m")
+    idx = as_packed(m_codes, m_scales, M, N, "m")
     if not isinstance(x_codes, torch.Tensor) or not isinstance(x_scales, torch.Tensor):
         raise TypeError("x_codes and x_scales must be torch.Tensors")
-    if x_codes.dim() == 0 or x_codes.shape[-1] != blocks_of(N) * BLOCK_BYTES:
+    *lead, row_bytes = x_codes.shape or (-1,)
+    if row_bytes != blocks_of(N) * BLOCK_BYTES:
         raise ValueError(f"packed rows of N={N} have {blocks_of(N) * BLOCK_BYTES} bytes each, got {tuple(x_codes.shape)}")
-    batch = 1
-    for s in x_codes.shape[:-1]:
-        batch *= s
-    as_packed(x_codes, x_scales, batch, N, "x")
-    if x_codes.device != m_codes.device:
+    batch = math.prod(lead)
+    if as_packed(x_codes, x_scales, batch, N, "x") != idx:
         raise ValueError("m and x must be on the same device")
-    out = _result(out, (*x_codes.shape[:-1], M), out_dtype, m_codes.device)
+    if out is not None:
+        _check_out(out, batch * M, out_dtype, x_codes.device)
+    else:
+        out = torch.empty(*lead, M, dtype=out_dtype, device=x_codes.device)
     if M and batch:
-        idx = m_codes.device.index
-        fn = _lib.load().feather_gemm_mxfp4
-        args = (m_codes.data_ptr(), m_scales.data_ptr(), x_codes.data_ptr(), x_scales.data_ptr(), out.data_ptr(), dst, M, N,
-                batch, _lib.current_stream_ptr(idx))
-        if torch.cuda.current_device() == idx:
-            _lib.check(fn(*args))
-        else:
-            with torch.cuda.device(idx):
-                _lib.check(fn(*args))
+        call(_lib.load().feather_gemm_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), x_codes.data_ptr(),
+                                                   x_scales.data_ptr(), out.data_ptr(), dst, M, N, batch))
     return out

@@ -14,7 +14,7 @@ import torch
 
 from .. import _lib
 from ..packers.fp8 import _tag, as_words
-from ..packers.mxfp4 import dtype_id
+from ..packers.mxfp4 import call, dtype_id
 
 __all__ = ["rotary_frequencies", "rotary_gpu"]
 
@@ -94,43 +94,40 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     dtype = dtype_id(x.dtype, "x")
     if not (x.is_cuda and positions.is_cuda and inv_freq.is_cuda):
         raise ValueError("x, positions and inv_freq must be CUDA tensors: feather_b200 has no CPU path")
-    if positions.device != x.device or inv_freq.device != x.device:
+    idx = x.get_device()
+    if positions.get_device() != idx or inv_freq.get_device() != idx:
         raise ValueError("x, positions and inv_freq must be on the same device")
     if x.dim() != 3:
         raise ValueError("x must be (tokens, heads, dim)")
     tokens, heads, dim = x.shape
-    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,) or not positions.is_contiguous():
+    wide = positions.dtype is torch.int64
+    if (not wide and positions.dtype is not torch.int32) or positions.shape != (tokens,) or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int64 or int32 tensor, one per token")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 vector")
     rotated = 2 * inv_freq.numel()
     if rotated < 2 or rotated > dim or rotated > MAX_ROTATED:
         raise ValueError(f"inv_freq turns {rotated} elements of heads of {dim} (at least 2, at most {MAX_ROTATED})")
     if mode is not None and dim % 4:
         raise ValueError("packed heads are whole words: dim must be a multiple of 4")
-    if x.numel() and x.stride(-1) != 1 and dim > 1:
+    token_stride, head_stride, last = x.stride()
+    total = tokens * heads * dim
+    if last != 1 and total:
         raise ValueError("the last dimension of x must be contiguous")
     given = out is not None
     if mode is None:
-        if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
-        elif (out.dtype != x.dtype or out.numel() != x.numel() or out.device != x.device or not out.is_contiguous()):
+        if not given:
+            out = torch.empty(tokens, heads, dim, dtype=x.dtype, device=x.device)
+        elif out.dtype != x.dtype or out.numel() != total or out.device != x.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor of x's type and size on its device")
-    elif out is None:
-        out = torch.empty((heads, tokens, dim // 4), dtype=torch.int32, device=x.device).view(torch.uint32)
+    elif not given:
+        out = torch.empty(heads, tokens, dim // 4, dtype=torch.uint32, device=x.device)
     else:
         out = as_words(out, "out")
-        if out.numel() != x.numel() // 4 or out.device != x.device:
+        if out.numel() != total // 4 or out.device != x.device:
             raise ValueError("out must hold heads * tokens * dim / 4 packed words on x's device")
-    if x.numel():
-        idx = x.device.index
-        fn = _lib.load().feather_rotary
-        args = (x.data_ptr(), dtype, x.stride(0), x.stride(1), positions.data_ptr(),
-                1 if positions.dtype == torch.int64 else 0, inv_freq.data_ptr(), out.data_ptr(), out_mode, tokens, heads,
-                dim, rotated, LAYOUTS[layout], float(scale), _lib.current_stream_ptr(idx))
-        if torch.cuda.current_device() == idx:
-            _lib.check(fn(*args))
-        else:
-            with torch.cuda.device(idx):
-                _lib.check(fn(*args))
+    if total:
+        call(_lib.load().feather_rotary, idx,
+             (x.data_ptr(), dtype, token_stride, head_stride, positions.data_ptr(), 1 if wide else 0, inv_freq.data_ptr(),
+              out.data_ptr(), out_mode, tokens, heads, dim, rotated, LAYOUTS[layout], float(scale)))
     return out if mode is None or given else _tag(out, mode)
