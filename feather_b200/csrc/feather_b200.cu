@@ -897,23 +897,22 @@ static int mx_decode_launch(const unsigned char* codes, const unsigned char* sca
     return launch_status();
 }
 
-template <int VT, int P, int R>
-static int mx_gemv_launch(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
-    auto kernel = mx_gemv_kernel<VT, P, R>;
-    a.chunk_blocks = kMgVecHalfs / (2 * P) / kMxBlock & ~3;
-    if (a.blocks < a.chunk_blocks) a.chunk_blocks = (a.blocks + 3) & ~3;
-    const int most = mg_smem_bytes<P>(kMgVecHalfs / (2 * P) / kMxBlock & ~3, 2 * P);
-    static std::atomic<unsigned long long> configured{0};
-    if (int st = ensure_smem(kernel, most, configured)) return st;
-    const int tiles = ((a.blocks < a.chunk_blocks ? a.blocks : a.chunk_blocks) + 3) / 4;
+template <int COLS, int ROWS, int STEP, typename K>
+static int mx_gemv_launch(K kernel, MxGemvArgs a, std::atomic<unsigned long long>& configured, const DeviceInfo& dev,
+                          cudaStream_t s) {
+    // ROWS: rows of a task, STEP: blocks of a row a warp takes at a time
+    constexpr int kMostBlocks = (kMgVecHalfs / COLS / kMxBlock) & ~7;
+    a.chunk_blocks = a.blocks < kMostBlocks ? (a.blocks + 7) & ~7 : kMostBlocks;
+    if (int st = ensure_smem(kernel, mg_smem_bytes(COLS, kMostBlocks, COLS, kMgPartFloats), configured)) return st;
+    const int steps = ((a.blocks < a.chunk_blocks ? a.blocks : a.chunk_blocks) + STEP - 1) / STEP;
     a.col_warps = kMgWarps;
-    while (a.col_warps > 1 && a.col_warps > tiles) a.col_warps >>= 1;
-    a.slots = kMgPartFloats / (a.col_warps * a.nv * 16 * R);
-    const long long groups = (a.M + 15) / 16;
+    while (a.col_warps > 1 && a.col_warps > steps) a.col_warps >>= 1;
+    a.slots = kMgPartFloats / (a.col_warps * a.nv * ROWS);
+    const long long units = STEP == 8 ? (a.M + 7) / 8 : (a.M + 15) / 16;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(groups < dev.sm_count ? groups : dev.sm_count));
+    cfg.gridDim = dim3((unsigned)(units < dev.sm_count ? units : dev.sm_count));
     cfg.blockDim = dim3(kMgThreads);
-    cfg.dynamicSmemBytes = mg_smem_bytes<P>(a.chunk_blocks, a.nv);
+    cfg.dynamicSmemBytes = mg_smem_bytes(COLS, a.chunk_blocks, a.nv, kMgPartFloats);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -923,11 +922,60 @@ static int mx_gemv_launch(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
 }
 
-template <int VT, int P>
-static int mx_gemv_rows(const MxGemvArgs& a, const DeviceInfo& dev, cudaStream_t s) {
-    if constexpr (P == 1)   // two groups at once need the registers of one column pair
-        if ((a.M + 15) / 16 > dev.sm_count) return mx_gemv_launch<VT, P, 2>(a, dev, s);
-    return mx_gemv_launch<VT, P, 1>(a, dev, s);
+template <int VT, int COLS, int R, bool WIDE>
+static int mx_gemv_line(const MxGemvArgs& a, const DeviceInfo& dev, cudaStream_t s) {
+    static std::atomic<unsigned long long> configured{0};
+    return mx_gemv_launch<COLS, 8 * R, 8>(mx_gemv_line_kernel<VT, COLS, R, WIDE>, a, configured, dev, s);
+}
+
+// kMgWarps x SLOTS x 4 KB of codes in flight, the vector chunk and partial sums in what is left.
+constexpr int kMrPartFloats = 4096;
+template <int VT, int COLS, int SLOTS, bool WHOLE>
+static int mx_gemv_ring(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
+    auto kernel = mx_gemv_ring_kernel<VT, COLS, SLOTS, WHOLE>;
+    constexpr int kRing = kMgWarps * SLOTS * kMrSlotBytes, kBars = kMgWarps * SLOTS * 8;
+    constexpr int kLeft = 227 * 1024 - kRing - kBars - mg_smem_bytes(COLS, 0, 0, kMrPartFloats);
+    constexpr int kMostBlocks = (kLeft / (COLS * (kMxBlock * 2 + 4))) & ~15;
+    a.chunk_blocks = a.blocks < kMostBlocks ? (a.blocks + 15) & ~15 : kMostBlocks;
+    a.part_floats = kMrPartFloats;
+    static std::atomic<unsigned long long> configured{0};
+    if (int st = ensure_smem(kernel, 227 * 1024, configured)) return st;
+    if (int st = status_word(&a.status)) return st;
+    const int spans = ((a.blocks < a.chunk_blocks ? a.blocks : a.chunk_blocks) + 15) / 16;
+    a.col_warps = kMgWarps;
+    while (a.col_warps > 1 && a.col_warps > spans) a.col_warps >>= 1;
+    a.slots = kMrPartFloats / (a.col_warps * a.nv * kMrRows);
+    CUtensorMap map;
+    if (!(WHOLE ? mr_make_map(&map, a.codes, 16ll * a.blocks, a.M) : atc_make_map(&map, a.codes, 16 * a.blocks, a.M, 128, kMrRows, true)))
+        return FEATHER_ERR_LAUNCH;
+    const long long groups = (a.M + kMrRows - 1) / kMrRows;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(groups < dev.sm_count ? groups : dev.sm_count));
+    cfg.blockDim = dim3(kMgThreads);
+    cfg.dynamicSmemBytes = kRing + kBars + mg_smem_bytes(COLS, a.chunk_blocks, a.nv, kMrPartFloats);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, map, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
+}
+
+template <int VT, int COLS>
+static int mx_gemv_cols(const MxGemvArgs& a, const DeviceInfo& dev, cudaStream_t s) {
+    if constexpr (COLS <= 2) {
+        if (a.M * a.blocks >= 128ll * dev.sm_count * (kMrSlotBytes / 16))
+            return a.blocks % 8 == 0 && aligned(a.scales, 2) ? mx_gemv_ring<VT, COLS, 2, true>(a, dev, s)
+                                                            : mx_gemv_ring<VT, COLS, 2, false>(a, dev, s);
+        const bool wide = a.blocks % 2 == 0 && aligned(a.codes, 32) && aligned(a.scales, 2);
+        const bool many = (a.M + 7) / 8 > dev.sm_count;   // two groups of rows at once where a CTA has them
+        return many ? (wide ? mx_gemv_line<VT, COLS, 2, true>(a, dev, s) : mx_gemv_line<VT, COLS, 2, false>(a, dev, s))
+                    : (wide ? mx_gemv_line<VT, COLS, 1, true>(a, dev, s) : mx_gemv_line<VT, COLS, 1, false>(a, dev, s));
+    } else {
+        static std::atomic<unsigned long long> configured{0};
+        return mx_gemv_launch<COLS, 16, 4>(mx_gemv_many_kernel<VT, COLS, 1>, a, configured, dev, s);
+    }
 }
 
 template <int VT>
@@ -938,9 +986,10 @@ static int mx_gemv(MxGemvArgs a, int batch, const DeviceInfo& dev, cudaStream_t 
     for (int b = 0; b < batch; b += most) {
         a.nv = batch - b < most ? batch - b : most;
         const int cols = a.nv * kParts;
-        const int st = cols <= 2   ? mx_gemv_rows<VT, 1>(a, dev, s)
-                       : cols <= 4 ? mx_gemv_rows<VT, 2>(a, dev, s)
-                                   : mx_gemv_rows<VT, 4>(a, dev, s);
+        const int st = cols == 1   ? mx_gemv_cols<VT, kParts == 1 ? 1 : 2>(a, dev, s)
+                       : cols == 2 ? mx_gemv_cols<VT, 2>(a, dev, s)
+                       : cols <= 4 ? mx_gemv_cols<VT, 4>(a, dev, s)
+                                   : mx_gemv_cols<VT, 8>(a, dev, s);
         if (st != FEATHER_OK) return st;
         a.v = reinterpret_cast<const unsigned char*>(a.v) + most * v_bytes;
         if (VT == kSrcMxfp4) a.v_scales += (long long)most * a.blocks;

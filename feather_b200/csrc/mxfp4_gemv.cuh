@@ -32,6 +32,7 @@
 // the CTA's rows are done; then the partials are added in warp order (same bits every run).
 // Loads go to registers, kMgDepth tiles of two groups ahead.
 #pragma once
+#include "attention_tc.cuh"   // tensor-map copies
 #include "gemv_common.cuh"
 #include "mxfp4_codec.cuh"
 
@@ -50,6 +51,20 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Two scale bytes (in the low half) to their values; the conversion gives 2^-127 and NaN their due.
+__device__ __forceinline__ float2 mx_scale_pair(uint32_t s) {
+    uint32_t d;
+    asm("{ .reg .b16 x; cvt.u16.u32 x, %1; cvt.rn.bf16x2.ue8m0x2 %0, x; }" : "=r"(d) : "r"(s));
+    return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xFFFF0000u));
+}
+
+// 32 bytes, 32-byte aligned.
+__device__ __forceinline__ void ldg_line(const uint4* p, uint32_t (&r)[8]) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
+}
+
 struct MxGemvArgs {
     const unsigned char* codes;
     const unsigned char* scales;
@@ -59,34 +74,100 @@ struct MxGemvArgs {
     long long M, N;
     int blocks;                      // per row
     int nv;                          // vectors of this launch
-    int chunk_blocks;                // blocks of the vector in shared memory at a time, a multiple of 4
+    int chunk_blocks;                // blocks of the vector in shared memory at a time, a multiple of 8
     int slots;                       // tasks whose partial sums fit
-    int col_warps;                   // warps that split a row's columns: a power of two, at most the first chunk's tiles
+    int part_floats;                 // room for partial sums
+    unsigned int* status;
+    int col_warps;                   // warps that split a row's columns: a power of two, at most the first chunk's tiles or lines
 };
 
-// Layout of dynamic shared memory: columns of halfs [2 P][chunk + 8], block scales
-// [nv][chunk_blocks], 64 bytes of zeros, partial sums.
-template <int P>
+// Layout of dynamic shared memory: COLS columns of chunk + 8 halfs, block scales [nv][chunk_blocks],
+// 64 bytes of zeros, partial sums.
 __host__ __device__ constexpr int mg_column(int chunk_blocks) { return chunk_blocks * kMxBlock + 8; }
-template <int P>
-__host__ __device__ constexpr int mg_smem_bytes(int chunk_blocks, int nv) {
-    return 2 * P * mg_column<P>(chunk_blocks) * 2 + 4 * nv * chunk_blocks + 64 + 4 * kMgPartFloats;
+__host__ __device__ constexpr int mg_smem_bytes(int cols, int chunk_blocks, int nv, int part_floats) {
+    return cols * mg_column(chunk_blocks) * 2 + 4 * nv * chunk_blocks + 64 + 4 * part_floats;
 }
 
-// VT: type of the vector (kSrc...); P: pairs of columns, 2 P columns in all; R: 16-row groups
-// a warp multiplies with the same vector registers.
-template <int VT, int P, int R>
+// Blocks [blk0, blk0 + pad_blk) of the vectors to shared memory, those from n_blk on as zeros: four
+// threads per block, eight elements each.
+template <int VT>
+__device__ __forceinline__ void mg_stage(const MxGemvArgs& a, __half* vec, float* vscale, int column, int blk0, int n_blk,
+                                         int pad_blk, int tid) {
+    constexpr int kParts = VT == kSrcF32 ? 2 : 1;
+    const int warp = tid >> 5, lane = tid & 31;
+                    const int quads = a.nv * pad_blk;
+                    for (int i0 = warp * 32; i0 < quads * 4; i0 += kMgThreads) {   // whole warps: the lanes shuffle
+                        const int i = i0 + lane, q = i & 3, b = (i >> 2) % pad_blk;
+                        const bool mine = (i >> 2) < quads;
+                        const int n = mine ? (i >> 2) / pad_blk : 0;
+                        const long long e0 = (long long)(blk0 + b) * kMxBlock + q * 8;
+                        float x[8];
+                        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+                        float sv = 1.f;
+                        if constexpr (VT == kSrcMxfp4) {
+                            if (b < n_blk) {
+                                const long long at = (long long)n * a.blocks + blk0 + b;
+                                mx_decode8(__ldg(reinterpret_cast<const uint32_t*>(a.v) + at * 4 + q), hi);
+                                sv = mx_scale_value(__ldg(a.v_scales + at));
+                            }
+                        } else {
+                            typedef typename MxElem<VT>::type E;
+                            const E* p = reinterpret_cast<const E*>(a.v) + (long long)n * a.N + e0;
+                            uint32_t top = 0u;
+                            if (e0 + 8 <= a.N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+                                mx_load8<VT>(p, 0, x);
+                            } else {
+    #pragma unroll
+                                for (int k = 0; k < 8; ++k) x[k] = e0 + k < a.N ? MxElem<VT>::get(p[k]) : 0.f;
+                            }
+    #pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const uint32_t u = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+                                if (u < 0x7F800000u) top = max(top, u);
+                            }
+                            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                            const uint32_t f = min(268u - (top >> 23), 253u);   // exponent field of the factor
+                            const float factor = __uint_as_float(f << 23);
+                            sv = __uint_as_float((254u - f) << 23);
+    #pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                float y[2], z[2];
+                                unsigned short w[2], l[2];
+    #pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    y[j] = x[2 * k + j] * factor;
+                                    w[j] = __half_as_ushort(__float2half_rn(y[j]));
+                                    z[j] = y[j] - __half2float(__ushort_as_half(w[j]));
+                                    l[j] = (w[j] & 0x7C00u) == 0x7C00u ? 0 : __half_as_ushort(__float2half_rn(z[j]));
+                                }
+                                hi[k] = w[0] | ((uint32_t)w[1] << 16);
+                                lo[k] = l[0] | ((uint32_t)l[1] << 16);
+                            }
+                        }
+                        if (!mine) continue;
+                        __half* d = vec + (long long)n * kParts * column + b * kMxBlock + q * 8;
+                        *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if (kParts == 2) *reinterpret_cast<uint4*>(d + column) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        if (q == 0) vscale[n * a.chunk_blocks + b] = sv;
+                    }
+}
+
+// VT: type of the vector (kSrc...); COLS: columns, 1, 2, 4 or 8 (an FP32 vector takes two); R:
+// 16-row groups a warp multiplies with the same vector registers.
+template <int VT, int COLS, int R>
 __global__ void __launch_bounds__(kMgThreads, 1)
-mx_gemv_kernel(const MxGemvArgs a) {
+mx_gemv_many_kernel(const MxGemvArgs a) {
     constexpr int kParts = VT == kSrcF32 ? 2 : 1;      // columns per vector
-    constexpr int kAcc = P * (kParts == 2 ? 1 : 2);    // vectors a launch can take
+    constexpr int kAcc = COLS / kParts;                // vectors a launch can take
+    constexpr int P = (COLS + 1) / 2;                  // products per 16 codes
     constexpr int kBuf = 3;                            // tiles in flight
     extern __shared__ __align__(16) unsigned char mg_smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int column = mg_column<P>(a.chunk_blocks);
+    const int column = mg_column(a.chunk_blocks);
     __half* vec = reinterpret_cast<__half*>(mg_smem);
-    float* vscale = reinterpret_cast<float*>(mg_smem + 2 * P * column * 2);
-    unsigned char* zeros = mg_smem + 2 * P * column * 2 + 4 * a.nv * a.chunk_blocks;
+    float* vscale = reinterpret_cast<float*>(mg_smem + COLS * column * 2);
+    unsigned char* zeros = mg_smem + COLS * column * 2 + 4 * a.nv * a.chunk_blocks;
     float* part = reinterpret_cast<float*>(zeros + 64);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -96,7 +177,9 @@ mx_gemv_kernel(const MxGemvArgs a) {
     const long long g_begin = groups * blockIdx.x / gridDim.x, g_end = groups * (blockIdx.x + 1) / gridDim.x;
     const int my_groups = (int)(g_end - g_begin);
     const int tasks = (my_groups + R - 1) / R;
-    const long long row_bytes = (long long)a.blocks * 16;
+    const int my_rows = (int)min(a.M - g_begin * 16, (long long)my_groups * 16);
+    const uint4* codes = reinterpret_cast<const uint4*>(a.codes) + g_begin * 16 * a.blocks;
+    const unsigned char* scales = a.scales + g_begin * 16 * a.blocks;
     if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0u;
 
     const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
@@ -111,28 +194,31 @@ mx_gemv_kernel(const MxGemvArgs a) {
             const int my_tasks = my_r < n_tasks ? (n_tasks - my_r + wr - 1) / wr : 0;
             const int steps = my_tasks * my_tiles;
 
-            // the matrix loads: tile `step` of this warp's walk (its tasks, inside them its tiles)
+            // The matrix loads, along this warp's walk (its tasks, inside them its tiles).  Offsets
+            // count from the CTA's first row in 32 bits.  Rows past the last are the last row again
+            // and blocks past the row's end its last block again: the former are not stored, the
+            // latter meet a vector of zeros.
             uint4 m[kBuf][R][2];
             uint32_t s[kBuf][R][2];
+            uint32_t row_at[R][2];
             int l_tile = 0, l_task = my_r;
             auto load = [&](int buf) {
-                const int blk = blk0 + (tile_begin + l_tile) * 4 + t;
-                const bool in_row = blk < blk0 + n_blk;
+                if (l_tile == 0) {
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const int grp = (first + l_task) * R + r;
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            row_at[r][h] = (uint32_t)min(((first + l_task) * R + r) * 16 + g + 8 * h, my_rows - 1) * (uint32_t)a.blocks;
+                }
+                const uint32_t blk = (uint32_t)(blk0 + min((tile_begin + l_tile) * 4 + t, n_blk - 1));
+#pragma unroll
+                for (int r = 0; r < R; ++r)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const long long row = (g_begin + grp) * 16 + g + 8 * h;
-                        const bool ok = in_row && grp < my_groups && row < a.M;
-                        m[buf][r][h] = make_uint4(0u, 0u, 0u, 0u);
-                        s[buf][r][h] = 0u;
-                        if (ok) {
-                            m[buf][r][h] = ldg_stream(reinterpret_cast<const uint4*>(a.codes + row * row_bytes) + blk);
-                            s[buf][r][h] = __ldg(a.scales + row * a.blocks + blk);
-                        }
+                        const uint32_t at = row_at[r][h] + blk;
+                        m[buf][r][h] = ldg_stream(codes + at);
+                        s[buf][r][h] = __ldg(scales + at);
                     }
-                }
                 if (++l_tile == my_tiles) l_tile = 0, l_task += wr;
             };
 #pragma unroll
@@ -142,63 +228,7 @@ mx_gemv_kernel(const MxGemvArgs a) {
             // the vector chunk: four threads per block, eight elements each
             if (ch > 0 || first > 0 ? chunks > 1 : true) {
                 if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
-                const int pad_blk = tiles * 4;
-                const int quads = a.nv * pad_blk;
-                for (int i0 = warp * 32; i0 < quads * 4; i0 += kMgThreads) {   // whole warps: the lanes shuffle
-                    const int i = i0 + lane, q = i & 3, b = (i >> 2) % pad_blk;
-                    const bool mine = (i >> 2) < quads;
-                    const int n = mine ? (i >> 2) / pad_blk : 0;
-                    const long long e0 = (long long)(blk0 + b) * kMxBlock + q * 8;
-                    float x[8];
-                    uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-                    float sv = 1.f;
-                    if constexpr (VT == kSrcMxfp4) {
-                        if (b < n_blk) {
-                            const long long at = (long long)n * a.blocks + blk0 + b;
-                            mx_decode8(__ldg(reinterpret_cast<const uint32_t*>(a.v) + at * 4 + q), hi);
-                            sv = mx_scale_value(__ldg(a.v_scales + at));
-                        }
-                    } else {
-                        typedef typename MxElem<VT>::type E;
-                        const E* p = reinterpret_cast<const E*>(a.v) + (long long)n * a.N + e0;
-                        uint32_t top = 0u;
-                        if (e0 + 8 <= a.N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-                            mx_load8<VT>(p, 0, x);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) x[k] = e0 + k < a.N ? MxElem<VT>::get(p[k]) : 0.f;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const uint32_t u = __float_as_uint(x[k]) & 0x7FFFFFFFu;
-                            if (u < 0x7F800000u) top = max(top, u);
-                        }
-                        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                        const uint32_t f = min(268u - (top >> 23), 253u);   // exponent field of the factor
-                        const float factor = __uint_as_float(f << 23);
-                        sv = __uint_as_float((254u - f) << 23);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float y[2], z[2];
-                            unsigned short w[2], l[2];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                y[j] = x[2 * k + j] * factor;
-                                w[j] = __half_as_ushort(__float2half_rn(y[j]));
-                                z[j] = y[j] - __half2float(__ushort_as_half(w[j]));
-                                l[j] = (w[j] & 0x7C00u) == 0x7C00u ? 0 : __half_as_ushort(__float2half_rn(z[j]));
-                            }
-                            hi[k] = w[0] | ((uint32_t)w[1] << 16);
-                            lo[k] = l[0] | ((uint32_t)l[1] << 16);
-                        }
-                    }
-                    if (!mine) continue;
-                    __half* d = vec + (long long)n * kParts * column + b * kMxBlock + q * 8;
-                    *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (kParts == 2) *reinterpret_cast<uint4*>(d + column) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    if (q == 0) vscale[n * a.chunk_blocks + b] = sv;
-                }
+                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, tiles * 4, tid);
                 __syncthreads();
             }
 
@@ -217,6 +247,19 @@ mx_gemv_kernel(const MxGemvArgs a) {
                             for (int n = 0; n < kAcc; ++n) acc[r][h][n] = 0.f;
                 }
                 const int b = (tile_begin + tile) * 4 + t;      // block inside the chunk
+                float2 sw[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) sw[r] = mx_scale_pair(s[buf][r][0] | (s[buf][r][1] << 8));
+                uint32_t x[R][2][4][4];                 // decoded once, multiplied with every pair of columns
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        mx_decode8(m[buf][r][h].x, x[r][h][0]);
+                        mx_decode8(m[buf][r][h].y, x[r][h][1]);
+                        mx_decode8(m[buf][r][h].z, x[r][h][2]);
+                        mx_decode8(m[buf][r][h].w, x[r][h][3]);
+                    }
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
                     const int col = 2 * p + (g & 1);
@@ -230,30 +273,30 @@ mx_gemv_kernel(const MxGemvArgs a) {
                         const uint4 bv = src[w];
 #pragma unroll
                         for (int r = 0; r < R; ++r) {
-                            uint32_t x[4], y[4];
-                            mx_decode8((&m[buf][r][0].x)[w], x);
-                            mx_decode8((&m[buf][r][1].x)[w], y);
-                            mma_f16(c[r], x[0], y[0], x[1], y[1], bv.x, bv.y);
-                            mma_f16(c[r], x[2], y[2], x[3], y[3], bv.z, bv.w);
+                            mma_f16(c[r], x[r][0][w][0], x[r][1][w][0], x[r][0][w][1], x[r][1][w][1], bv.x, bv.y);
+                            mma_f16(c[r], x[r][0][w][2], x[r][1][w][2], x[r][0][w][3], x[r][1][w][3], bv.z, bv.w);
                         }
                     }
+                    // (a block's sum) x (the vector block's power of two) x (the matrix block's)
+                    if constexpr (kParts == 2) {
+                        const float sv = p < a.nv ? vscale[p * a.chunk_blocks + b] : 0.f;
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
+                        for (int r = 0; r < R; ++r) {
+                            acc[r][0][p] = fmaf((c[r][0] + c[r][1]) * sv, sw[r].x, acc[r][0][p]);
+                            acc[r][1][p] = fmaf((c[r][2] + c[r][3]) * sv, sw[r].y, acc[r][1][p]);
+                        }
+                    } else {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float sw = mx_scale_value(s[buf][r][h]);
-                            if constexpr (kParts == 2) {
-                                const float sv = p < a.nv ? vscale[p * a.chunk_blocks + b] : 0.f;
-                                acc[r][h][p] = fmaf((c[r][2 * h] + c[r][2 * h + 1]) * sv, sw, acc[r][h][p]);
-                            } else {
+                        for (int e = 0; e < (COLS > 1 ? 2 : 1); ++e) {
+                            const int n = 2 * p + e;
+                            const float sv = n < a.nv ? vscale[n * a.chunk_blocks + b] : 0.f;
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const int n = 2 * p + e;
-                                    const float sv = n < a.nv ? vscale[n * a.chunk_blocks + b] : 0.f;
-                                    acc[r][h][n] = fmaf(c[r][2 * h + e] * sv, sw, acc[r][h][n]);
-                                }
+                            for (int r = 0; r < R; ++r) {
+                                acc[r][0][n] = fmaf(c[r][e] * sv, sw[r].x, acc[r][0][n]);
+                                acc[r][1][n] = fmaf(c[r][2 + e] * sv, sw[r].y, acc[r][1][n]);
                             }
                         }
+                    }
                 }
                 if (++tile == my_tiles) {
                     // the row's partial sums: over the four lanes, then one slot per warp
@@ -293,6 +336,398 @@ mx_gemv_kernel(const MxGemvArgs a) {
             float x = 0.f;
             for (int k = 0; k < wk; ++k) x += part[((task * wk + k) * a.nv + n) * (16 * R) + r];
             if (grp < my_groups && row < a.M) a.out[n * a.M + row] = x;
+        }
+        __syncthreads();
+    }
+}
+
+// One or two columns (a vector, an FP32 vector in two parts, two vectors).  A lane takes 32 bytes of
+// a row, two neighbouring blocks, and the four lanes of a row a whole 128-byte line: half the lines
+// per load instruction.  The product's rows 0-7 are the first blocks of eight rows, its rows 8-15
+// the second blocks of the same rows; column n holds the vector for block n of the line, zero but
+// in the slots of lane n / 2.  Of the four sums a lane gets back, the first is its first block's and
+// the last its second block's.  WIDE: 32-byte loads (rows of an even number of blocks).
+template <int VT, int COLS, int R, bool WIDE>
+__global__ void __launch_bounds__(kMgThreads, 1)
+mx_gemv_line_kernel(const MxGemvArgs a) {
+    constexpr int kParts = VT == kSrcF32 ? 2 : 1;
+    constexpr int kAcc = COLS / kParts;
+    constexpr int kBuf = R == 1 ? 6 : 4;
+    extern __shared__ __align__(16) unsigned char mg_smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int column = mg_column(a.chunk_blocks);
+    __half* vec = reinterpret_cast<__half*>(mg_smem);
+    float* vscale = reinterpret_cast<float*>(mg_smem + COLS * column * 2);
+    unsigned char* zeros = mg_smem + COLS * column * 2 + 4 * a.nv * a.chunk_blocks;
+    float* part = reinterpret_cast<float*>(zeros + 64);
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const long long groups = (a.M + 7) / 8;
+    const long long g_begin = groups * blockIdx.x / gridDim.x, g_end = groups * (blockIdx.x + 1) / gridDim.x;
+    const int my_groups = (int)(g_end - g_begin);
+    const int tasks = (my_groups + R - 1) / R;
+    const int my_rows = (int)min(a.M - g_begin * 8, (long long)my_groups * 8);
+    const uint4* codes = reinterpret_cast<const uint4*>(a.codes) + g_begin * 8 * a.blocks;
+    const unsigned char* scales = a.scales + g_begin * 8 * a.blocks;
+    if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0u;
+
+    const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
+    const int wk = a.col_warps, wr = kMgWarps / wk, my_k = warp & (wk - 1), my_r = warp / wk;
+    for (int first = 0; first < tasks; first += a.slots) {
+        const int n_tasks = min(a.slots, tasks - first);
+        for (int ch = 0; ch < chunks; ++ch) {
+            const int blk0 = ch * a.chunk_blocks, n_blk = min(a.chunk_blocks, a.blocks - blk0);
+            const int lines = (n_blk + 7) / 8;
+            const int line_begin = lines * my_k / wk, my_lines = lines * (my_k + 1) / wk - line_begin;
+            const int my_tasks = my_r < n_tasks ? (n_tasks - my_r + wr - 1) / wr : 0;
+            const int steps = my_tasks * my_lines;
+
+            // The matrix loads, along this warp's walk (its tasks, inside them its lines).  Offsets
+            // count from the CTA's first row in 32 bits.  Rows past the last are the last row again
+            // and blocks past the row's end its last blocks again: the former are not stored, the
+            // latter meet a vector of zeros.
+            uint32_t m[kBuf][R][8];
+            uint32_t s[kBuf][R];
+            uint32_t row_at[R];
+            int l_line = 0, l_task = my_r;
+            auto load = [&](int buf) {
+                if (l_line == 0) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        row_at[r] = (uint32_t)min(((first + l_task) * R + r) * 8 + g, my_rows - 1) * (uint32_t)a.blocks;
+                }
+                const int blk = (line_begin + l_line) * 8 + 2 * t;
+                const uint32_t b0 = (uint32_t)(blk0 + min(blk, WIDE ? n_blk - 2 : n_blk - 1));
+                const uint32_t b1 = (uint32_t)(blk0 + min(blk + 1, n_blk - 1));
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if constexpr (WIDE) {
+                        ldg_line(codes + row_at[r] + b0, m[buf][r]);
+                        s[buf][r] = __ldg(reinterpret_cast<const unsigned short*>(scales + row_at[r] + b0));
+                    } else {
+                        const uint4 x = ldg_stream(codes + row_at[r] + b0), y = ldg_stream(codes + row_at[r] + b1);
+                        m[buf][r][0] = x.x; m[buf][r][1] = x.y; m[buf][r][2] = x.z; m[buf][r][3] = x.w;
+                        m[buf][r][4] = y.x; m[buf][r][5] = y.y; m[buf][r][6] = y.z; m[buf][r][7] = y.w;
+                        s[buf][r] = __ldg(scales + row_at[r] + b0) | ((uint32_t)__ldg(scales + row_at[r] + b1) << 8);
+                    }
+                }
+                if (++l_line == my_lines) l_line = 0, l_task += wr;
+            };
+#pragma unroll
+            for (int i = 0; i < kBuf - 1; ++i)
+                if (i < steps) load(i);
+
+            if (ch > 0 || first > 0 ? chunks > 1 : true) {
+                if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
+                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, lines * 8, tid);
+                __syncthreads();
+            }
+
+            float acc[R][kAcc];
+            int line = 0, task = my_r;
+            const bool diag = (g >> 1) == t;        // this lane's column is of one of its own blocks
+            auto multiply = [&](int buf) {
+                if (line == 0) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int n = 0; n < kAcc; ++n) acc[r][n] = 0.f;
+                }
+                const int b = (line_begin + line) * 8;      // the line's first block inside the chunk
+                const uint4* src[COLS];
+                float c[R][COLS][4];
+#pragma unroll
+                for (int p = 0; p < COLS; ++p) {
+                    src[p] = reinterpret_cast<const uint4*>(
+                        diag ? reinterpret_cast<const unsigned char*>(vec + p * column + (b + g) * kMxBlock) : zeros);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) c[r][p][0] = c[r][p][1] = c[r][p][2] = c[r][p][3] = 0.f;
+                }
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint4 bv[COLS];
+#pragma unroll
+                    for (int p = 0; p < COLS; ++p) bv[p] = src[p][w];
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        uint32_t x[4], y[4];
+                        mx_decode8(m[buf][r][w], x);
+                        mx_decode8(m[buf][r][4 + w], y);
+#pragma unroll
+                        for (int p = 0; p < COLS; ++p) {
+                            mma_f16(c[r][p], x[0], y[0], x[1], y[1], bv[p].x, bv[p].y);
+                            mma_f16(c[r][p], x[2], y[2], x[3], y[3], bv[p].z, bv[p].w);
+                        }
+                    }
+                }
+                // (a block's sum) x (the vector block's power of two) x (the matrix block's)
+#pragma unroll
+                for (int n = 0; n < kAcc; ++n) {
+                    const float2 sv = *reinterpret_cast<const float2*>(vscale + n * a.chunk_blocks + b + 2 * t);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float2 sw = mx_scale_pair(s[buf][r]);
+                        const float c0 = kParts == 2 ? c[r][0][0] + c[r][COLS - 1][0] : c[r][n][0];
+                        const float c1 = kParts == 2 ? c[r][0][3] + c[r][COLS - 1][3] : c[r][n][3];
+                        acc[r][n] = fmaf(c0 * sv.x, sw.x, acc[r][n]);
+                        acc[r][n] = fmaf(c1 * sv.y, sw.y, acc[r][n]);
+                    }
+                }
+                if (++line == my_lines) {
+                    // the row's partial sums: over the four lanes, then one slot per warp
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int n = 0; n < kAcc; ++n) {
+                            float x = acc[r][n];
+                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+                            if (t == 0) {
+                                float* to = part + ((task * wk + my_k) * kAcc + n) * (8 * R) + r * 8 + g;
+                                *to = ch == 0 ? x : *to + x;
+                            }
+                        }
+                    line = 0;
+                    task += wr;
+                }
+            };
+            for (int i = 0; i < steps; i += kBuf) {
+#pragma unroll
+                for (int u = 0; u < kBuf; ++u) {
+                    if (i + u < steps) {
+                        if (i + u + kBuf - 1 < steps) load((u + kBuf - 1) % kBuf);
+                        multiply(u);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < n_tasks * kAcc * 8 * R; i += kMgThreads) {
+            const int r = i % (8 * R), n = (i / (8 * R)) % kAcc, task = i / (8 * R * kAcc);
+            const int row = (first + task) * R * 8 + r;
+            float x = 0.f;
+            for (int k = 0; k < wk; ++k) x += part[((task * wk + k) * kAcc + n) * (8 * R) + r];
+            if (row < my_rows) a.out[n * a.M + g_begin * 8 + row] = x;
+        }
+        __syncthreads();
+    }
+}
+
+// Large matrices: the line kernel's arithmetic with the codes coming through shared memory.  A warp
+// owns kMrSlots slots of 4 KB, 16 rows x 512 codes (two lines), that it fills itself with
+// tensor-map copies (128-byte swizzle: the reads below are free of bank conflicts); it refills a
+// slot as soon as it has read it, so nothing is shared and nothing but arrival is waited for.
+// Loads to registers (the line kernel) keep far fewer bytes in flight than their count suggests.
+constexpr int kMrRows = 16, kMrLines = 2, kMrSlotBytes = kMrRows * kMrLines * 128;
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// Host side: rows of whole lines as {128 bytes, rows, lines} with boxes of 16 rows x 2 lines.
+inline bool mr_make_map(CUtensorMap* map, const void* base, long long row_bytes, long long rows) {
+    const AtcEncodeTiled encode = atc_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {128, (cuuint64_t)rows, (cuuint64_t)(row_bytes / 128)};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, 128};
+    const cuuint32_t box[3] = {128, kMrRows, kMrLines};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// WHOLE: rows of whole lines, one three-dimensional copy per slot; else two two-dimensional ones.
+// Shared memory: slots, then as above, then a barrier per slot.
+template <int VT, int COLS, int SLOTS, bool WHOLE>
+__global__ void __launch_bounds__(kMgThreads, 1)
+mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a) {
+    constexpr int kParts = VT == kSrcF32 ? 2 : 1;
+    constexpr int kAcc = COLS / kParts;
+    constexpr int R = kMrRows / 8;
+    extern __shared__ __align__(1024) unsigned char mr_smem[];
+    unsigned char* mg_smem = mr_smem + kMgWarps * SLOTS * kMrSlotBytes;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int column = mg_column(a.chunk_blocks);
+    __half* vec = reinterpret_cast<__half*>(mg_smem);
+    float* vscale = reinterpret_cast<float*>(mg_smem + COLS * column * 2);
+    unsigned char* zeros = mg_smem + COLS * column * 2 + 4 * a.nv * a.chunk_blocks;
+    float* part = reinterpret_cast<float*>(zeros + 64);
+    const uint32_t slots = smem_u32(mr_smem) + warp * (SLOTS * kMrSlotBytes);
+    const uint32_t bars = smem_u32(part + a.part_floats) + warp * (SLOTS * 8);
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (smem_u32(mr_smem) & 1023u) {                 // every CTA alike
+        if (tid == 0) atomicOr(a.status, 2u);
+        return;
+    }
+    if (lane == 0) {
+        for (int i = 0; i < SLOTS; ++i) mbar_init(bars + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const long long groups = (a.M + kMrRows - 1) / kMrRows;
+    const int g_begin = (int)(groups * blockIdx.x / gridDim.x), tasks = (int)(groups * (blockIdx.x + 1) / gridDim.x) - g_begin;
+    const int my_rows = (int)min(a.M - (long long)g_begin * kMrRows, (long long)tasks * kMrRows);
+    const unsigned char* scales = a.scales + (long long)g_begin * kMrRows * a.blocks;
+    if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0u;
+
+    const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
+    const int wk = a.col_warps, wr = kMgWarps / wk, my_k = warp & (wk - 1), my_r = warp / wk;
+    bool ok = true;
+    int used = 0;                                    // slots filled so far, over all chunks
+    for (int first = 0; first < tasks; first += a.slots) {
+        const int n_tasks = min(a.slots, tasks - first);
+        for (int ch = 0; ch < chunks; ++ch) {
+            const int blk0 = ch * a.chunk_blocks, n_blk = min(a.chunk_blocks, a.blocks - blk0);
+            const int spans = (n_blk + 8 * kMrLines - 1) / (8 * kMrLines);
+            const int span_begin = spans * my_k / wk, my_spans = spans * (my_k + 1) / wk - span_begin;
+            const int my_tasks = my_r < n_tasks ? (n_tasks - my_r + wr - 1) / wr : 0;
+            const int steps = my_tasks * my_spans;
+
+            int l_span = 0, l_task = my_r;
+            auto fill = [&](int slot) {              // the next step of this warp's walk; one lane
+                const int y = (g_begin + first + l_task) * kMrRows, z = blk0 / 8 + (span_begin + l_span) * kMrLines;
+                const uint32_t to = slots + slot * kMrSlotBytes, bar = bars + 8 * slot;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar, kMrSlotBytes);
+                    if constexpr (WHOLE) {
+                        tma_load_3d(to, &map, 0, y, z, bar);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kMrLines; ++i) tma_load_2d(to + i * (kMrRows * 128), &map, (z + i) * 128, y, bar);
+                    }
+                }
+                if (++l_span == my_spans) l_span = 0, l_task += wr;
+            };
+            for (int i = 0; i < SLOTS && i < steps; ++i) fill((used + i) % SLOTS);
+
+            // scale bytes of a step, two blocks of two lines of R rows, a step ahead
+            uint32_t s[kMrLines][R], s_next[kMrLines][R];
+            int s_span = 0, s_task = my_r;
+            auto load_scales = [&]() {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const uint32_t row = (uint32_t)min((first + s_task) * kMrRows + r * 8 + g, my_rows - 1) * (uint32_t)a.blocks;
+#pragma unroll
+                    for (int l = 0; l < kMrLines; ++l) {
+                        const int blk = ((span_begin + s_span) * kMrLines + l) * 8 + 2 * t;
+                        if constexpr (WHOLE) {
+                            const int at = min(blk, n_blk - 2);
+                            s_next[l][r] = __ldg(reinterpret_cast<const unsigned short*>(scales + row + blk0 + at));
+                        } else {
+                            s_next[l][r] = __ldg(scales + row + blk0 + min(blk, n_blk - 1)) |
+                                           ((uint32_t)__ldg(scales + row + blk0 + min(blk + 1, n_blk - 1)) << 8);
+                        }
+                    }
+                }
+                if (++s_span == my_spans) s_span = 0, s_task += wr;
+            };
+            if (steps > 0) load_scales();
+
+            if (ch > 0 || first > 0 ? chunks > 1 : true) {
+                if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
+                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, spans * 8 * kMrLines, tid);
+                __syncthreads();
+            }
+
+            float acc[R][kAcc];
+            int span = 0, task = my_r;
+            const bool diag = (g >> 1) == t;
+            for (int i = 0; i < steps; ++i, ++used) {
+                const int slot = used % SLOTS;
+                if (span == 0) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int n = 0; n < kAcc; ++n) acc[r][n] = 0.f;
+                }
+#pragma unroll
+                for (int l = 0; l < kMrLines; ++l)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) s[l][r] = s_next[l][r];
+                if (i + 1 < steps) load_scales();
+                ok = ok && mbar_wait(bars + 8 * slot, (uint32_t)((used / SLOTS) & 1), a.status);
+                const unsigned char* from = mr_smem + (warp * SLOTS + slot) * kMrSlotBytes + g * 128;
+#pragma unroll
+                for (int l = 0; l < kMrLines; ++l) {
+                    const int b = ((span_begin + span) * kMrLines + l) * 8;      // the line's first block inside the chunk
+                    float c[R][COLS][4];
+                    const uint4* src[COLS];
+#pragma unroll
+                    for (int p = 0; p < COLS; ++p) {
+                        src[p] = reinterpret_cast<const uint4*>(
+                            diag ? reinterpret_cast<const unsigned char*>(vec + p * column + (b + g) * kMxBlock) : zeros);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) c[r][p][0] = c[r][p][1] = c[r][p][2] = c[r][p][3] = 0.f;
+                    }
+                    uint4 m[R][2];
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)      // 16-byte units of a row are swizzled with the row's number
+                            m[r][h] = *reinterpret_cast<const uint4*>(from + l * (kMrRows * 128) + r * 1024 + (((2 * t + h) ^ g) << 4));
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint4 bv[COLS];
+#pragma unroll
+                        for (int p = 0; p < COLS; ++p) bv[p] = src[p][w];
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            uint32_t x[4], y[4];
+                            mx_decode8(w == 0 ? m[r][0].x : w == 1 ? m[r][0].y : w == 2 ? m[r][0].z : m[r][0].w, x);
+                            mx_decode8(w == 0 ? m[r][1].x : w == 1 ? m[r][1].y : w == 2 ? m[r][1].z : m[r][1].w, y);
+#pragma unroll
+                            for (int p = 0; p < COLS; ++p) {
+                                mma_f16(c[r][p], x[0], y[0], x[1], y[1], bv[p].x, bv[p].y);
+                                mma_f16(c[r][p], x[2], y[2], x[3], y[3], bv[p].z, bv[p].w);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < kAcc; ++n) {
+                        const float2 sv = *reinterpret_cast<const float2*>(vscale + n * a.chunk_blocks + b + 2 * t);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            const float2 sw = mx_scale_pair(s[l][r]);
+                            const float c0 = kParts == 2 ? c[r][0][0] + c[r][COLS - 1][0] : c[r][n][0];
+                            const float c1 = kParts == 2 ? c[r][0][3] + c[r][COLS - 1][3] : c[r][n][3];
+                            acc[r][n] = fmaf(c0 * sv.x, sw.x, acc[r][n]);
+                            acc[r][n] = fmaf(c1 * sv.y, sw.y, acc[r][n]);
+                        }
+                    }
+                }
+                __syncwarp();                        // every lane has read the slot
+                if (i + SLOTS < steps) fill(slot);
+                if (++span == my_spans) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int n = 0; n < kAcc; ++n) {
+                            float x = acc[r][n];
+                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+                            if (t == 0) {
+                                float* to = part + ((task * wk + my_k) * kAcc + n) * kMrRows + r * 8 + g;
+                                *to = ch == 0 ? x : *to + x;
+                            }
+                        }
+                    span = 0;
+                    task += wr;
+                }
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < n_tasks * kAcc * kMrRows; i += kMgThreads) {
+            const int r = i % kMrRows, n = (i / kMrRows) % kAcc, task = i / (kMrRows * kAcc);
+            const int row = (first + task) * kMrRows + r;
+            float x = 0.f;
+            for (int k = 0; k < wk; ++k) x += part[((task * wk + k) * kAcc + n) * kMrRows + r];
+            if (row < my_rows) a.out[n * a.M + (long long)g_begin * kMrRows + row] = x;
         }
         __syncthreads();
     }
