@@ -59,7 +59,8 @@ SYMBOLS = {
     "feather_dot_fp8_static_max_words": (_i64, []),
     "feather_encode_mxfp4": (_i32, [_vp, _i32, _vp, _vp, _i64, _i64, _vp]),
     "feather_decode_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _vp]),
-    "feather_gemv_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "feather_gemv_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "feather_gemv_mxfp4_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "feather_gemm_mxfp4": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp]),
     "feather_rotary": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32,
                               ctypes.c_float, _vp]),

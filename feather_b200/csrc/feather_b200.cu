@@ -57,6 +57,7 @@ struct Tuning {
     std::atomic<int> ring_pre_kb_e4m3{-1};
     std::atomic<int> attn_tc{1};
     std::atomic<int> multi_tc{1};
+    std::atomic<int> mx_digits{1};
 };
 static Tuning g_tune;
 
@@ -82,6 +83,7 @@ static int apply_tuning(const char* spec) {
         else if (is("ring_pre_kb_e4m3") && val >= -1 && val <= 16384) g_tune.ring_pre_kb_e4m3 = (int)val;
         else if (is("attn_tc") && val >= 0 && val <= 2) g_tune.attn_tc = (int)val;
         else if (is("multi_tc") && (val == 0 || val == 1)) g_tune.multi_tc = (int)val;
+        else if (is("mx_digits") && val >= 0 && val <= 2) g_tune.mx_digits = (int)val;
         else return FEATHER_ERR_BAD_ARG;
         p = end;
     }
@@ -998,47 +1000,118 @@ static int mx_gemv(MxGemvArgs a, int batch, const DeviceInfo& dev, cudaStream_t 
     return FEATHER_OK;
 }
 
-template <int NT, int CHAINS, int OUT>
-static int mx_gemm_launch(const unsigned char* m_codes, const unsigned char* x_codes, MxGemmArgs a, const DeviceInfo& dev,
-                          cudaStream_t s) {
-    typedef GmLayout<NT, CHAINS> L;
-    auto kernel = mx_gemm_kernel<NT, CHAINS, OUT>;
+template <int NT, int OUT, bool DIGITS>
+static int mx_gemm_launch(const unsigned char* x_codes, MxGemmArgs a, const DeviceInfo& dev, cudaStream_t s) {
+    typedef GmLayout<NT> L;
+    auto kernel = mx_gemm_kernel<NT, OUT, DIGITS>;
     static std::atomic<unsigned long long> configured{0};
     if (int st = ensure_smem(kernel, L::kBytes, configured)) return st;
     if (int st = status_word(&a.status)) return st;
-    CUtensorMap map_m, map_x;
-    if (!atc_make_map(&map_m, m_codes, a.blocks * 16, a.M, kGmBox, kGmRows, true) ||
-        !atc_make_map(&map_x, x_codes, a.blocks * 16, a.batch, kGmBox, NT, true))
-        return FEATHER_ERR_LAUNCH;
-    constexpr int kSize = OUT == kSrcF32 ? 4 : 2;
-    CUtensorMap map_out = {};
-    a.bulk = (long long)a.M * kSize % 16 == 0 && aligned(a.out, 16);
-    if (a.bulk && !gm_make_out_map(&map_out, a.out, kSize, OUT == kSrcBF16, a.M, a.batch, kGmPiece / (32 * kSize)))
-        return FEATHER_ERR_LAUNCH;
     a.tiles_m = (a.M + kGmRows - 1) / kGmRows;
     a.tiles_x = (a.batch + NT - 1) / NT;
     const long long tiles = (long long)a.tiles_m * a.tiles_x;
     if (tiles > 0x7FFFFFFFll - dev.sm_count) return FEATHER_ERR_TOO_LARGE;
+    // A stage takes about 0.23 us of an SM whose operands come from HBM, joining the partial sums
+    // about 1.8 us: split rows of at least 16 stages while the CTAs still run at once.  (Clusters
+    // of 8 do not: 16 of them took two waves, 10.6 against 6.6 us at 2048 x 5632 x 16.)
+    const int stages = (a.blocks + kGmBlocks - 1) / kGmBlocks;
+    a.split = 1;
+    while (a.split < 4 && stages >= 16 && tiles * a.split * 2 <= dev.sm_count) a.split *= 2;
+    CUtensorMap map_m, map_x, map_out = {};
+    constexpr int kSize = OUT == kSrcF32 ? 4 : 2;
+    a.bulk = !DIGITS && a.split == 1 && (long long)a.M * kSize % 16 == 0 && aligned(a.out, 16);
+    if (!atc_make_map(&map_m, a.m_codes, a.blocks * 16, a.M, kGmBox, kGmRows, true) ||
+        !atc_make_map(&map_x, x_codes, a.blocks * 16, a.batch, kGmBox, NT, true) ||
+        (a.bulk && !gm_make_out_map(&map_out, a.out, kSize, OUT == kSrcBF16, a.M, a.batch, kGmPiece / (32 * kSize))))
+        return FEATHER_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles < dev.sm_count ? tiles : dev.sm_count));
+    cfg.gridDim = dim3((unsigned)((tiles < dev.sm_count ? tiles : dev.sm_count) * a.split));
     cfg.blockDim = dim3(kGmThreads);
     cfg.dynamicSmemBytes = L::kBytes;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = a.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, map_m, map_x, map_out, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
 }
 
+static int mx_scale_align(const void* m_scales, const void* x_scales, int blocks) {
+    return blocks % 16 == 0 && aligned(m_scales, 16) && aligned(x_scales, 16) ? 16
+           : blocks % 4 == 0 && aligned(m_scales, 4) && aligned(x_scales, 4)  ? 4
+                                                                              : 1;
+}
+
+// Which vectors go through the product kernel.
+static bool mx_wants_digits(long long M, long long N, int batch, int v_dtype) {
+    const int knob = g_tune.mx_digits.load(std::memory_order_relaxed);
+    (void)batch; (void)v_dtype;
+    return knob == 2 || (knob == 1 && M * N >= (8ll << 20));
+}
+
+// Tiles of 224 or of 128 rows of x: those whose waves take less, a wave of the wide ones taking
+// 1.5 times as long (measured at 16384 x 8192 x 4096: 219 and 350 us for 17 and 28 waves).
+static bool mx_wide_tiles(const MxGemmArgs& a, const DeviceInfo& dev) {
+    if (a.batch <= 128) return false;
+    const long long tm = (a.M + kGmRows - 1) / kGmRows;
+    const long long wide = (tm * ((a.batch + 223) / 224) + dev.sm_count - 1) / dev.sm_count;
+    const long long narrow = (tm * ((a.batch + 127) / 128) + dev.sm_count - 1) / dev.sm_count;
+    return 3 * wide < 2 * narrow;
+}
+
 template <int OUT>
-static int mx_gemm(const unsigned char* m_codes, const unsigned char* x_codes, const MxGemmArgs& a, const DeviceInfo& dev,
-                   cudaStream_t s) {
-    return a.batch <= 32    ? mx_gemm_launch<32, 1, OUT>(m_codes, x_codes, a, dev, s)
-           : a.batch <= 64  ? mx_gemm_launch<64, 1, OUT>(m_codes, x_codes, a, dev, s)
-           : a.batch <= 128 ? mx_gemm_launch<128, 1, OUT>(m_codes, x_codes, a, dev, s)
-                            : mx_gemm_launch<224, 1, OUT>(m_codes, x_codes, a, dev, s);
+static int mx_gemm(const unsigned char* x_codes, const MxGemmArgs& a, const DeviceInfo& dev, cudaStream_t s) {
+    return a.batch <= 16    ? mx_gemm_launch<16, OUT, false>(x_codes, a, dev, s)
+           : a.batch <= 32  ? mx_gemm_launch<32, OUT, false>(x_codes, a, dev, s)
+           : a.batch <= 64  ? mx_gemm_launch<64, OUT, false>(x_codes, a, dev, s)
+           : mx_wide_tiles(a, dev) ? mx_gemm_launch<224, OUT, false>(x_codes, a, dev, s)
+                                   : mx_gemm_launch<128, OUT, false>(x_codes, a, dev, s);
+}
+
+// Dense vectors as digits, eight at a time, through the product kernel.  `workspace` holds the
+// digits of one launch: 16 codes rows per vector, then their scales.
+static long long mx_digits_bytes(int blocks, int vectors) { return (long long)vectors * kGmDigits * blocks * 17; }
+template <int VT>
+static int mx_gemv_digits(const MxGemvArgs& v, int batch, unsigned char* workspace, const DeviceInfo& dev, cudaStream_t s) {
+    MxGemmArgs a = {};
+    a.m_codes = v.codes;
+    a.m_scales = v.scales;
+    a.M = (int)v.M;
+    a.blocks = v.blocks;
+    a.v_dtype = VT;
+    a.N = v.N;
+    for (int b = 0; b < batch; b += 8) {
+        const int nv = batch - b < 8 ? batch - b : 8;
+        unsigned char* scales = workspace + (long long)nv * kGmDigits * v.blocks * 16;
+        a.v = reinterpret_cast<const unsigned char*>(v.v) + b * v.N * (VT == kSrcF32 ? 4 : 2);
+        a.out = v.out + b * v.M;
+        a.x_scales = scales;
+        a.batch = nv * kGmDigits;
+        a.align = mx_scale_align(a.m_scales, scales, a.blocks);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((4ll * v.blocks * nv + 255) / 256));
+        cfg.blockDim = dim3(256);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, mx_digits_kernel<VT>, a.v, reinterpret_cast<uint32_t*>(workspace), scales,
+                               (long long)v.N, v.blocks, nv) != cudaSuccess)
+            return FEATHER_ERR_LAUNCH;
+        const int st = nv == 1   ? mx_gemm_launch<16, kSrcF32, true>(workspace, a, dev, s)
+                       : nv == 2 ? mx_gemm_launch<32, kSrcF32, true>(workspace, a, dev, s)
+                       : nv <= 4 ? mx_gemm_launch<64, kSrcF32, true>(workspace, a, dev, s)
+                                 : mx_gemm_launch<128, kSrcF32, true>(workspace, a, dev, s);
+        if (st != FEATHER_OK) return st;
+    }
+    return FEATHER_OK;
 }
 
 template <int T, int MODE>
@@ -1665,8 +1738,13 @@ int feather_decode_mxfp4(const uint8_t* codes, const uint8_t* scales, void* dst,
                                           : mx_decode_launch<kSrcBF16>(codes, scales, dst, rows, cols, *dev, s);
 }
 
+int64_t feather_gemv_mxfp4_workspace_bytes(int64_t M, int64_t N, int batch, int v_dtype) {
+    if (M < 0 || N < 0 || batch < 0 || N > kMxMaxCols || v_dtype == FEATHER_SRC_MXFP4 || !mx_wants_digits(M, N, batch, v_dtype)) return 0;
+    return mx_digits_bytes(mx_blocks(N), batch < 8 ? batch : 8);
+}
+
 int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const void* v, int v_dtype, const uint8_t* v_scales,
-                       float* out, int64_t M, int64_t N, int batch, void* stream) {
+                       float* out, void* workspace, int64_t M, int64_t N, int batch, void* stream) {
     if (M < 0 || N < 0 || batch < 0) return FEATHER_ERR_BAD_ARG;
     if (v_dtype < 0 || v_dtype > FEATHER_SRC_MXFP4) return FEATHER_ERR_MODE;
     if (M == 0 || batch == 0) return FEATHER_OK;
@@ -1692,6 +1770,26 @@ int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const vo
     a.M = M;
     a.N = N;
     a.blocks = mx_blocks(N);
+    if (!packed && mx_wants_digits(M, N, batch, v_dtype)) {
+        if (!workspace) return FEATHER_ERR_WORKSPACE;
+        if (!aligned(workspace, 16)) return FEATHER_ERR_MISALIGNED;
+        unsigned char* w = static_cast<unsigned char*>(workspace);
+        return v_dtype == FEATHER_SRC_F16   ? mx_gemv_digits<kSrcF16>(a, batch, w, *dev, s)
+               : v_dtype == FEATHER_SRC_F32 ? mx_gemv_digits<kSrcF32>(a, batch, w, *dev, s)
+                                            : mx_gemv_digits<kSrcBF16>(a, batch, w, *dev, s);
+    }
+    if (packed && mx_wants_digits(M, N, batch, v_dtype)) {
+        MxGemmArgs x = {};
+        x.m_codes = m_codes;
+        x.m_scales = m_scales;
+        x.x_scales = v_scales;
+        x.out = out;
+        x.M = (int)M;
+        x.batch = batch;
+        x.blocks = a.blocks;
+        x.align = mx_scale_align(m_scales, v_scales, a.blocks);
+        return mx_gemm<kSrcF32>(static_cast<const unsigned char*>(v), x, *dev, s);
+    }
     switch (v_dtype) {
         case FEATHER_SRC_F16: return mx_gemv<kSrcF16>(a, batch, *dev, s);
         case FEATHER_SRC_F32: return mx_gemv<kSrcF32>(a, batch, *dev, s);
@@ -1719,18 +1817,17 @@ int feather_gemm_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const ui
     if (N == 0)
         return cudaMemsetAsync(out, 0, (size_t)M * batch * size, s) == cudaSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
     MxGemmArgs a = {};
+    a.m_codes = m_codes;
     a.m_scales = m_scales;
     a.x_scales = x_scales;
     a.out = out;
     a.M = (int)M;
     a.batch = (int)batch;
     a.blocks = mx_blocks(N);
-    a.align = a.blocks % 16 == 0 && aligned(m_scales, 16) && aligned(x_scales, 16) ? 16
-              : a.blocks % 4 == 0 && aligned(m_scales, 4) && aligned(x_scales, 4) ? 4
-                                                                                   : 1;
-    return out_dtype == FEATHER_SRC_F16   ? mx_gemm<kSrcF16>(m_codes, x_codes, a, *dev, s)
-           : out_dtype == FEATHER_SRC_F32 ? mx_gemm<kSrcF32>(m_codes, x_codes, a, *dev, s)
-                                          : mx_gemm<kSrcBF16>(m_codes, x_codes, a, *dev, s);
+    a.align = mx_scale_align(m_scales, x_scales, a.blocks);
+    return out_dtype == FEATHER_SRC_F16   ? mx_gemm<kSrcF16>(x_codes, a, *dev, s)
+           : out_dtype == FEATHER_SRC_F32 ? mx_gemm<kSrcF32>(x_codes, a, *dev, s)
+                                          : mx_gemm<kSrcBF16>(x_codes, a, *dev, s);
 }
 
 int feather_rotary(const void* x, int dtype, int64_t token_stride, int64_t head_stride, const void* positions,

@@ -18,6 +18,15 @@
 // Warps: 0 copies, 1 issues, 2-5 scales, 6-9 store finished tiles while the next one is
 // multiplied (two accumulators alternate).  Every wait is bounded; a CTA that gave up
 // frees its tensor memory.
+//
+// Few tiles: a cluster of 2 or 4 CTAs shares one tile, each with its part of the row; the
+// partial sums meet through distributed shared memory and are added in rank order, each CTA
+// storing its share of the columns.  No scratch in global memory, the same bits every run.
+//
+// Dense vectors (DIGITS): a vector is first written as kGmDigits packed rows whose sum it is --
+// each row is the quantised remainder of the ones before it (mx_digits_kernel), at least two more
+// bits per row -- and its columns are added when they are stored.  With a matrix that is read
+// once anyway the extra columns cost nothing, and nothing of the matrix is decoded.
 #pragma once
 #include "attention_tc.cuh"   // descriptors, tensor-map copies, tensor-memory loads
 #include "mxfp4_codec.cuh"
@@ -33,21 +42,20 @@ constexpr int kGmGroup = 4;                    // stages whose scales travel tog
 constexpr int kGmPiece = 2048;                 // bytes of a warp's piece of the result: 32 rows of m x 32 (16-bit) or 16 of x
 constexpr int kGmOutBytes = 4 * 2 * kGmPiece;  // two per storing warp
 
-template <int NT, int CHAINS>
+template <int NT>
 struct GmLayout {
     static constexpr int kRowAtoms = NT > 128 ? 2 : 1;                     // 128-row pieces of x's scales
     static constexpr int kA = kGmRows * kGmBox, kB = NT * kGmBox;          // operand bytes of a stage
     static constexpr int kSfStage = 2 * (1 + kRowAtoms) * 512;             // scale bytes of a stage: 2 x (m, x)
     static constexpr int kSfGroup = kGmGroup * kSfStage;
     static constexpr int kMost = (227 * 1024 - 256 - 2 * kSfGroup - kGmOutBytes) / (kA + kB);
-    static constexpr int kStages = kMost > 8 ? 8 : kMost;
+    static constexpr int kStages = kMost > 10 ? 10 : kMost;
     static constexpr int kSf = kStages * (kA + kB);                        // two groups of scales behind the operands
     static constexpr int kOut = kSf + 2 * kSfGroup;                        // pieces of the result on their way out
     static constexpr int kBar = kOut + kGmOutBytes;
     static constexpr int kBytes = kBar + 8 * (2 * kStages + 8) + 16;
-    static constexpr int kAccCols = NT * CHAINS;
     static constexpr int kSfColsA = 2 * 4, kSfColsB = 2 * 4 * kRowAtoms;   // 32-bit columns of a stage's scales
-    static constexpr int kSfCol = 2 * kAccCols;                            // two sets alternate
+    static constexpr int kSfCol = 2 * NT;                                  // two sets alternate
     static constexpr int kCols = 512;
     static_assert(kSfCol + 2 * (kSfColsA + kSfColsB) <= kCols, "tensor memory");
     static_assert(kA % 1024 == 0 && kB % 1024 == 0, "swizzled tiles are 1 KiB aligned");
@@ -107,7 +115,9 @@ inline bool gm_make_out_map(CUtensorMap* map, void* out, int out_size, bool bf16
 }
 
 // The scale bytes of blocks [k, k + 32) of a row as eight words, those past the row's end as 0.
-__device__ __forceinline__ void gm_load_scales(uint32_t (&w)[8], const unsigned char* row, int k, int blocks, int align) {
+// `all` is one past the last scale byte of the operand.
+__device__ __forceinline__ void gm_load_scales(uint32_t (&w)[8], const unsigned char* row, int k, int blocks, int align,
+                                               const unsigned char* begin, const unsigned char* all) {
     if (align == 16) {                           // whole rows in steps of 16 blocks
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -118,12 +128,30 @@ __device__ __forceinline__ void gm_load_scales(uint32_t (&w)[8], const unsigned 
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = k + 4 * i < blocks ? __ldg(reinterpret_cast<const uint32_t*>(row + k) + i) : 0u;
     } else {
+        // any alignment: the aligned words that cover the bytes, shifted into place
+        const unsigned char* from = reinterpret_cast<const unsigned char*>(reinterpret_cast<uintptr_t>(row + k) & ~(uintptr_t)3);
+        const uint32_t shift = 8u * (uint32_t)(reinterpret_cast<uintptr_t>(row + k) & 3);
+        const int left = blocks - k;             // bytes of this row still wanted, at least 1
+        uint32_t x[9];
+#pragma unroll
+        for (int i = 0; i < 9; ++i) {
+            const unsigned char* p = from + 4 * i;
+            x[i] = 0u;
+            if (4 * i < left + 3) {
+                if (p >= begin && p + 4 <= all) {
+                    x[i] = __ldg(reinterpret_cast<const uint32_t*>(p));
+                } else {                         // a word across an end of the operand
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (p + b >= begin && p + b < all) x[i] |= (uint32_t)__ldg(p + b) << (8 * b);
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w[i] = 0u;
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (k + 4 * i + b < blocks) w[i] |= (uint32_t)__ldg(row + k + 4 * i + b) << (8 * b);
+            w[i] = __funnelshift_r(x[i], x[i + 1], shift);
+            const int over = 4 * i + 4 - left;   // bytes of this word past the row's end
+            if (over > 0) w[i] = over >= 4 ? 0u : w[i] & (0xFFFFFFFFu >> (8 * over));
         }
     }
 }
@@ -134,16 +162,119 @@ struct MxGemmArgs {
     void* out;                    // batch x M
     int M, batch, blocks;
     int tiles_m, tiles_x;
+    int split;                    // CTAs of a cluster that share a tile
     int align;                    // of the scale rows: 16, 4 or 1
     int bulk;                     // 1: result rows are 16-byte aligned, pieces leave by tensor-map copies
     unsigned int* status;
+    // dense vectors: x is their digits, batch counts digit rows; what the rare repair needs
+    const unsigned char* m_codes;
+    const void* v;
+    int v_dtype;
+    long long N;
 };
 
-template <int NT, int CHAINS, int OUT>
+constexpr int kGmDigits = 16;
+
+// Dense vectors to digits: row 16 n + d of (codes, scales) is the quantised remainder of vector n
+// after d rows.  Four threads per block, eight elements each; the remainder is exact in FP32 (an
+// element and its code's value are within a factor of two, or the code is zero).  After
+// kGmDigits rows it is at most 2^-32 of the block's largest element.  A block with an infinity
+// or a NaN gets scale 255 in row 0.
+template <int VT>
+__global__ void __launch_bounds__(256)
+mx_digits_kernel(const void* __restrict__ v, uint32_t* __restrict__ codes, unsigned char* __restrict__ scales, long long N,
+                 int blocks, int vectors) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    typedef typename MxElem<VT>::type E;
+    const int quads = blocks * vectors, i = blockIdx.x * blockDim.x + threadIdx.x;
+    const bool mine = (i >> 2) < quads;
+    const int q = i & 3, n = mine ? (i >> 2) / blocks : 0, b = mine ? (i >> 2) - n * blocks : 0;
+    const long long e0 = (long long)b * kMxBlock + q * 8;
+    const E* p = reinterpret_cast<const E*>(v) + n * N + e0;
+    float x[8];
+    if (e0 + 8 <= N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        mx_load8<VT>(p, 0, x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = e0 + k < N ? MxElem<VT>::get(p[k]) : 0.f;
+    }
+#pragma unroll 4
+    for (int d = 0; d < kGmDigits; ++d) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const uint32_t s = mx_scale_byte(top);
+        const float f = mx_to_grid(s), back = mx_scale_value(s);
+        float y[8];
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = x[k] * f;
+        const uint32_t c = s == 255u ? 0u : mx_encode8(y);
+        mx_decode8(c, h);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 z = h2_to_f2(h[k]);
+            x[2 * k] = s == 255u ? 0.f : x[2 * k] - z.x * back;
+            x[2 * k + 1] = s == 255u ? 0.f : x[2 * k + 1] - z.y * back;
+        }
+        if (mine) {
+            const long long at = ((long long)n * kGmDigits + d) * blocks + b;
+            codes[at * 4 + q] = c;
+            if (q == 0) scales[at] = (unsigned char)s;
+        }
+    }
+}
+
+// The digits' columns of a vector added up, the smallest digit first.
+__device__ __forceinline__ float gm_add_digits(uint32_t taddr) {
+    float r[kGmDigits];
+    tmem_ld<kGmDigits>(taddr, r);
+    float x = r[kGmDigits - 1];
+#pragma unroll
+    for (int d = kGmDigits - 2; d >= 0; --d) x += r[d];
+    return x;
+}
+// Bit c: vector x0 + c holds an infinity or a NaN (its first digits have a block of scale 255).
+template <int VECTORS>
+__device__ __forceinline__ uint32_t gm_find_not_finite(const MxGemmArgs& g, int x0, int lane) {
+    uint32_t found = 0u;
+    for (int c = 0; c < VECTORS && (x0 + c) * kGmDigits < g.batch; ++c) {
+        const unsigned char* s = g.x_scales + (long long)(x0 + c) * kGmDigits * g.blocks;
+        bool bad = false;
+        for (int b = lane; b < g.blocks; b += 32) bad |= __ldg(s + b) == 255;
+        if (__any_sync(0xFFFFFFFFu, bad)) found |= 1u << c;
+    }
+    return found;
+}
+// Row m times such a vector: the blocks that hold what is not finite decide the result.
+__device__ __noinline__ float gm_not_finite(const MxGemmArgs& g, int m, int n) {
+    const unsigned char* s = g.x_scales + (long long)n * kGmDigits * g.blocks;
+    float sum = 0.f;
+    for (int b = 0; b < g.blocks; ++b) {
+        if (s[b] != 255) continue;
+        const float scale = mx_scale_value(g.m_scales[(long long)m * g.blocks + b]);
+        for (int i = 0; i < kMxBlock && (long long)b * kMxBlock + i < g.N; ++i) {
+            const long long e = n * g.N + (long long)b * kMxBlock + i;
+            const float v = g.v_dtype == kSrcF32   ? reinterpret_cast<const float*>(g.v)[e]
+                            : g.v_dtype == kSrcF16 ? MxElem<kSrcF16>::get(reinterpret_cast<const unsigned short*>(g.v)[e])
+                                                   : MxElem<kSrcBF16>::get(reinterpret_cast<const unsigned short*>(g.v)[e]);
+            const uint32_t pair = g.m_codes[((long long)m * g.blocks + b) * 16 + i / 2];
+            uint32_t h[4];
+            mx_decode8(i & 1 ? pair >> 4 : pair, h);
+            sum = fmaf(h2_to_f2(h[0]).x * scale, v, sum);
+        }
+    }
+    return sum;
+}
+
+template <int NT, int OUT, bool DIGITS>
 __global__ void __launch_bounds__(kGmThreads, 1)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant__ CUtensorMap map_x,
                const __grid_constant__ CUtensorMap map_out, const MxGemmArgs g) {
-    typedef GmLayout<NT, CHAINS> L;
+    typedef GmLayout<NT> L;
     extern __shared__ __align__(1024) unsigned char gm_smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t sbase = smem_u32(gm_smem), bars = sbase + L::kBar;
@@ -184,23 +315,29 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     asm volatile("griddepcontrol.wait;" ::: "memory");   // operands and result may be the previous kernel's
 
     const int n_tiles = g.tiles_m * g.tiles_x;
-    const int n_step = (g.blocks + kGmBlocks - 1) / kGmBlocks;
+    const int all_steps = (g.blocks + kGmBlocks - 1) / kGmBlocks;
+    // this CTA's tiles, and its part of their rows in stages: pairs of stages dealt to the cluster
+    const int rank = (int)blockIdx.x % g.split, tile0 = (int)blockIdx.x / g.split, tile_step = (int)gridDim.x / g.split;
+    const int pairs = (all_steps + 1) / 2;
+    const int k_begin = 2 * (pairs * rank / g.split);
+    const int n_step = min(2 * (pairs * (rank + 1) / g.split), all_steps) - k_begin;
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
             int it = 0;
-            for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
+            for (int tile = tile0; tile < n_tiles && ok; tile += tile_step) {
                 const int m0 = (tile / g.tiles_x) * kGmRows, x0 = (tile % g.tiles_x) * NT;
                 for (int k = 0; k < n_step && ok; ++k, ++it) {
                     const int s = it % L::kStages;
                     if (it >= L::kStages) ok = mbar_wait(empty(s), (uint32_t)((it / L::kStages - 1) & 1), g.status);
                     mbar_arrive_expect_tx(full(s), (uint32_t)(L::kA + L::kB));
                     const uint32_t at = sbase + s * (L::kA + L::kB);
-                    tma_load_2d(at, &map_m, k * kGmBox, m0, full(s));
-                    tma_load_2d(at + L::kA, &map_x, k * kGmBox, x0, full(s));
+                    tma_load_2d(at, &map_m, (k_begin + k) * kGmBox, m0, full(s));
+                    tma_load_2d(at + L::kA, &map_x, (k_begin + k) * kGmBox, x0, full(s));
                 }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         // The whole warp walks the stages (uniform control flow and addresses); one elected lane issues.
         const bool leader = elect_one();
@@ -208,7 +345,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         int s = 0, done = 0, grp = 0;          // ring slot, tiles, scale groups so far
         uint32_t phase = 0;
         const uint64_t desc_a = tc_desc_swizzled(sbase, 1024, 2), desc_sf = tc_desc(sbase + L::kSf, 128, 128);
-        for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x, ++done) {
+        for (int tile = tile0; tile < n_tiles && ok; tile += tile_step, ++done) {
             const int a = done & 1;
             if (done >= 2) ok = mbar_wait(acc_empty(a), (uint32_t)((done / 2 - 1) & 1), g.status);
             for (int k = 0; k < n_step && ok; ++k) {
@@ -219,7 +356,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
                 const uint64_t at = desc_a + (uint32_t)(s * ((L::kA + L::kB) / 16));
                 const uint64_t sf = desc_sf + (uint32_t)((grp & 1) * (L::kSfGroup / 16) + (k % kGmGroup) * (L::kSfStage / 16));
                 const uint32_t sfa = tmem + L::kSfCol + (k & 1) * (L::kSfColsA + L::kSfColsB), sfb = sfa + L::kSfColsA;
-                const uint32_t d = tmem + NT * (CHAINS * a + k % CHAINS);
+                const uint32_t d = tmem + NT * a;
                 const bool last = k == n_step - 1;
                 if (leader) {
 #pragma unroll
@@ -227,7 +364,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         gm_mma(d, at + 2 * j, at + L::kA / 16 + 2 * j, j & 1 ? gm_idesc<NT>(2) : gm_idesc<NT>(0),
-                               sfa + 4 * (j / 2), sfb + 4 * L::kRowAtoms * (j / 2), k >= CHAINS || j > 0);
+                               sfa + 4 * (j / 2), sfb + 4 * L::kRowAtoms * (j / 2), k > 0 || j > 0);
                     tc_commit(empty(s));
                     if (k % kGmGroup == kGmGroup - 1 || last) tc_commit(sf_empty(grp & 1));
                     if (last) tc_commit(acc_full(a));
@@ -242,6 +379,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         // issued behind the fence of this one: the fence would wait for them.
         const int i = tid - 64;
         const int at = (i & 31) * 16 + (i >> 5) * 4;
+        const unsigned char* m_all = g.m_scales + (long long)g.M * g.blocks;
+        const unsigned char* x_all = g.x_scales + (long long)g.batch * g.blocks;
         uint32_t q[1 + L::kRowAtoms][8];
         auto load = [&](int tile, int k) {
             const int m = (tile / g.tiles_x) * kGmRows + i, x = (tile % g.tiles_x) * NT + i;
@@ -252,7 +391,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
                 if (there && mine) {
                     const unsigned char* row = p == 0 ? g.m_scales + (long long)m * g.blocks
                                                       : g.x_scales + (long long)(x + 128 * (p - 1)) * g.blocks;
-                    gm_load_scales(q[p], row, k * kGmBlocks, g.blocks, g.align);
+                    gm_load_scales(q[p], row, (k_begin + k) * kGmBlocks, g.blocks, g.align, p == 0 ? g.m_scales : g.x_scales,
+                                   p == 0 ? m_all : x_all);
                 } else {
 #pragma unroll
                     for (int w = 0; w < 8; ++w) q[p][w] = 0u;
@@ -261,8 +401,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
         };
         bool ok = true;
         int grp = 0;
-        load(blockIdx.x, 0);
-        for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
+        load(tile0, 0);
+        for (int tile = tile0; tile < n_tiles && ok; tile += tile_step) {
             for (int k = 0; k < n_step && ok; k += kGmGroup, ++grp) {
                 if (grp >= 2) ok = mbar_wait(sf_empty(grp & 1), (uint32_t)((grp / 2 - 1) & 1), g.status);
                 unsigned char* sf = gm_smem + L::kSf + (grp & 1) * L::kSfGroup + at;
@@ -278,62 +418,132 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sf_full(grp & 1));
                 if (k + kGmGroup < n_step) load(tile, k + kGmGroup);
-                else load(tile + gridDim.x, 0);
+                else load(tile + tile_step, 0);
             }
         }
-    } else {
-        const int w = warp & 3;                  // the quarter of tensor memory this warp can read
-        typedef typename MxElem<OUT>::type E;
+    }
+    typedef typename MxElem<OUT>::type E;
+    constexpr int kSums = DIGITS ? NT / kGmDigits : NT;      // results of a row of m in a tile
+    E* out = reinterpret_cast<E*>(g.out);
+    const int w = warp & 3;                      // the quarter of tensor memory a storing warp can read
+    const int sums_all = DIGITS ? g.batch / kGmDigits : g.batch;
+    uint32_t repair = 0u;                        // vectors of this tile that hold an infinity or a NaN
+    if (warp >= 6 && g.split == 1) {
         constexpr int kPiece = kGmPiece / (32 * (int)sizeof(E));
-        E* out = reinterpret_cast<E*>(g.out);
         int done = 0, pieces = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x, ++done) {
+        for (int tile = tile0; tile < n_tiles && ok; tile += tile_step, ++done) {
             const int a = done & 1;
-            const int m = (tile / g.tiles_x) * kGmRows + w * 32 + lane, x0 = (tile % g.tiles_x) * NT;
+            const int m = (tile / g.tiles_x) * kGmRows + w * 32 + lane, x0 = (tile % g.tiles_x) * kSums;
+            if (DIGITS) repair = gm_find_not_finite<kSums>(g, x0, lane);
             ok = mbar_wait(acc_full(a), (uint32_t)((done / 2) & 1), g.status);
             ok = __all_sync(0xFFFFFFFFu, ok);
             tc_fence_after();
+            const uint32_t from = tmem + NT * a + ((uint32_t)(w * 32) << 16);
+            if constexpr (DIGITS) {
 #pragma unroll 1
-            for (int c = 0; c < NT; c += kPiece) {
-                if (x0 + c >= g.batch) break;
-                float r[kPiece];
-                const uint32_t from = tmem + NT * CHAINS * a + c + ((uint32_t)(w * 32) << 16);
-                tmem_ld<kPiece>(from, r);
-#pragma unroll
-                for (int h = 1; h < CHAINS; ++h) {
-                    if (h < n_step) {            // the chains that this row length reaches
-                        float more[kPiece];
-                        tmem_ld<kPiece>(from + NT * h, more);
-#pragma unroll
-                        for (int v = 0; v < kPiece; ++v) r[v] += more[v];
+                for (int c = 0; c < kSums; ++c) {
+                    if (x0 + c >= sums_all) break;
+                    float r = gm_add_digits(from + kGmDigits * c);
+                    if (ok && m < g.M) {
+                        if ((repair >> c) & 1) r = gm_not_finite(g, m, x0 + c);
+                        out[(long long)(x0 + c) * g.M + m] = r;
                     }
                 }
-                if (g.bulk) {
-                    // [kPiece rows of x][32 of m] through shared memory; rows outside the result are not written
-                    const uint32_t at = L::kOut + (w * 2 + (pieces & 1)) * kGmPiece;
-                    E* to = reinterpret_cast<E*>(gm_smem + at) + lane;
-                    if (lane == 0) bulk_wait_read<1>();      // the piece before the last has been read
-                    __syncwarp();
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < NT; c += kPiece) {
+                    if (x0 + c >= g.batch) break;
+                    float r[kPiece];
+                    tmem_ld<kPiece>(from + c, r);
+                    if (g.bulk) {
+                        // [kPiece rows of x][32 of m] through shared memory; rows outside the result are not written
+                        const uint32_t at = L::kOut + (w * 2 + (pieces & 1)) * kGmPiece;
+                        E* to = reinterpret_cast<E*>(gm_smem + at) + lane;
+                        if (lane == 0) bulk_wait_read<1>();      // the piece before the last has been read
+                        __syncwarp();
 #pragma unroll
-                    for (int v = 0; v < kPiece; ++v) to[32 * v] = MxElem<OUT>::put(r[v]);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0 && ok && m - lane < g.M) tma_store_2d(&map_out, sbase + at, m - lane, x0 + c);
-                    if (lane == 0) bulk_commit();
-                    ++pieces;
-                } else if (ok && m < g.M) {
-                    E* to = out + (long long)(x0 + c) * g.M + m;
+                        for (int v = 0; v < kPiece; ++v) to[32 * v] = MxElem<OUT>::put(r[v]);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0 && ok && m - lane < g.M) tma_store_2d(&map_out, sbase + at, m - lane, x0 + c);
+                        if (lane == 0) bulk_commit();
+                        ++pieces;
+                    } else if (ok && m < g.M) {
+                        E* to = out + (long long)(x0 + c) * g.M + m;
 #pragma unroll
-                    for (int v = 0; v < kPiece; ++v)
-                        if (x0 + c + v < g.batch) to[(long long)v * g.M] = MxElem<OUT>::put(r[v]);
+                        for (int v = 0; v < kPiece; ++v)
+                            if (x0 + c + v < g.batch) to[(long long)v * g.M] = MxElem<OUT>::put(r[v]);
+                    }
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty(a));
         }
-        if (lane == 0) bulk_wait<0>();           // shared memory and the result outlive the copies
+        if (!DIGITS && lane == 0) bulk_wait<0>();           // shared memory and the result outlive the copies
+    }
+    if (g.split > 1) {
+        // One tile per cluster.  Column c of the result is rank c % split's: every CTA sends its partial
+        // sums there, to [c / split][sender][128 rows] in the place of the operands, which
+        // every CTA's products have read behind the first barrier.  Stores, not loads: nothing waits
+        // for a round trip.
+        const int m = (tile0 / g.tiles_x) * kGmRows + w * 32 + lane, x0 = (tile0 % g.tiles_x) * kSums;
+        const int sums = min(kSums, sums_all - x0);
+        const uint32_t part = sbase + (w * 32 + lane) * 4;
+        bool ok = true;
+        if (warp >= 6) {
+            if (DIGITS) repair = gm_find_not_finite<kSums>(g, x0, lane);
+            ok = mbar_wait(acc_full(0), 0u, g.status);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            tc_fence_after();
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 6) {
+            const uint32_t from = tmem + ((uint32_t)(w * 32) << 16);
+            const uint32_t row = (uint32_t)rank * (kGmRows * 4), shift = (uint32_t)(31 - __clz(g.split));
+            if constexpr (DIGITS) {
+                for (int c = 0; c < sums; ++c)
+                    st_cluster_f32(map_cluster(part + ((uint32_t)(c >> shift) << shift) * (kGmRows * 4) + row, (uint32_t)(c & (g.split - 1))),
+                                   gm_add_digits(from + kGmDigits * c));
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < NT; c += 16) {
+                    if (c >= sums) break;
+                    float r[16];
+                    tmem_ld<16>(from + c, r);
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (c + v < sums)
+                            st_cluster_f32(map_cluster(part + ((uint32_t)((c + v) >> shift) << shift) * (kGmRows * 4) + row,
+                                                       (uint32_t)((c + v) & (g.split - 1))), r[v]);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 6) {
+            const float* mine = reinterpret_cast<const float*>(gm_smem) + w * 32 + lane;
+            const int n_mine = (sums - rank + g.split - 1) / g.split;
+            for (int i = 0; i < n_mine; i += 8) {        // eight columns at a time: their loads overlap
+                float r[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[e] = i + e < n_mine ? mine[(i + e) * g.split * kGmRows] : 0.f;
+                for (int p = 1; p < g.split; ++p)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (i + e < n_mine) r[e] += mine[((i + e) * g.split + p) * kGmRows];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = rank + (i + e) * g.split;
+                    if (i + e < n_mine && ok && m < g.M) {
+                        if (DIGITS && ((repair >> c) & 1)) r[e] = gm_not_finite(g, m, x0 + c);
+                        out[(long long)(x0 + c) * g.M + m] = MxElem<OUT>::put(r[e]);
+                    }
+                }
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();

@@ -76,8 +76,11 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
     else:
         out = torch.empty(batch, M, dtype=torch.float32, device=v.device)
     if M and batch:
-        call(_lib.load().feather_gemv_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype,
-                                                   scales_ptr, out.data_ptr(), M, N, batch))
+        lib = _lib.load()
+        need = lib.feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype) if scales_ptr is None else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
+        call(lib.feather_gemv_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr,
+                                           out.data_ptr(), ws.data_ptr() if need else None, M, N, batch))
     return out
 
 

@@ -538,10 +538,14 @@ int feather_decode_mxfp4(const uint8_t* codes, const uint8_t* scales, void* dst,
  *   v         batch x N values of v_dtype, contiguous, or FEATHER_SRC_MXFP4:
  *             packed codes with v_scales (ignored otherwise)
  *   out       batch x M floats
+ *   workspace feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype) bytes, 16-byte
+ *             aligned, contents irrelevant; may be NULL where that is 0.  Calls
+ *             that can overlap need one each
  */
 int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const void* v, int v_dtype,
-                       const uint8_t* v_scales, float* out, int64_t M, int64_t N, int batch,
-                       void* stream);
+                       const uint8_t* v_scales, float* out, void* workspace, int64_t M, int64_t N,
+                       int batch, void* stream);
+int64_t feather_gemv_mxfp4_workspace_bytes(int64_t M, int64_t N, int batch, int v_dtype);
 
 /*
  * out[b][r] = sum_j value(m[r][j]) * value(x[b][j]), both operands packed

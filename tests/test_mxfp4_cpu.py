@@ -52,11 +52,11 @@ def test_c_entry_points_refuse_before_any_device_call(lib):
     assert enc(odd, 0, p, p, 1, 5, None) == -2 and enc(p, 0, p + 8, p, 1, 5, None) == -2
     assert dec(p, p, p + 2, 1, 1, 5, None) == -2 and dec(p + 1, p, p, 1, 1, 5, None) == -2
     assert enc(p, 0, p, p, 1, 1 << 31, None) == -8
-    assert gemv(p, p, p, 0, None, p, 0, 8, 1, None) == 0 and gemv(p, p, p, 0, None, p, 8, 8, 0, None) == 0
-    assert gemv(p, p, p, 4, None, p, 8, 8, 1, None) == -3 and gemv(p, p, p, 0, None, p, 8, -8, 1, None) == -1
-    assert gemv(p, p, p, 3, None, p, 8, 8, 1, None) == -1            # a packed vector without its scales
-    assert gemv(p, p, p, 0, None, p, 8, 8, 65, None) == -8
-    assert gemv(p + 1, p, p, 0, None, p, 8, 8, 1, None) == -2 and gemv(p, p, p + 2, 3, p, p, 8, 8, 1, None) == -2
+    assert gemv(p, p, p, 0, None, p, None, 0, 8, 1, None) == 0 and gemv(p, p, p, 0, None, p, None, 8, 8, 0, None) == 0
+    assert gemv(p, p, p, 4, None, p, None, 8, 8, 1, None) == -3 and gemv(p, p, p, 0, None, p, None, 8, -8, 1, None) == -1
+    assert gemv(p, p, p, 3, None, p, None, 8, 8, 1, None) == -1            # a packed vector without its scales
+    assert gemv(p, p, p, 0, None, p, None, 8, 8, 65, None) == -8
+    assert gemv(p + 1, p, p, 0, None, p, None, 8, 8, 1, None) == -2 and gemv(p, p, p + 2, 3, p, p, None, 8, 8, 1, None) == -2
     assert gemm(p, p, p, p, p, 3, 8, 8, 8, None) == -3 and gemm(p, p, p, p, None, 0, 8, 8, 8, None) == -1
     assert gemm(p, p, p, p, p, 0, 0, 8, 8, None) == 0 and gemm(p, None, p, p, p, 0, 8, 8, 8, None) == -1
     assert gemm(p, p, p + 8, p, p, 0, 8, 8, 8, None) == -2 and gemm(p, p, p, p, odd, 0, 8, 8, 8, None) == -2
