@@ -57,7 +57,6 @@ struct Tuning {
     std::atomic<int> ring_pre_kb_e4m3{-1};
     std::atomic<int> attn_tc{1};
     std::atomic<int> multi_tc{1};
-    std::atomic<int> mx_digits{1};
 };
 static Tuning g_tune;
 
@@ -83,7 +82,6 @@ static int apply_tuning(const char* spec) {
         else if (is("ring_pre_kb_e4m3") && val >= -1 && val <= 16384) g_tune.ring_pre_kb_e4m3 = (int)val;
         else if (is("attn_tc") && val >= 0 && val <= 2) g_tune.attn_tc = (int)val;
         else if (is("multi_tc") && (val == 0 || val == 1)) g_tune.multi_tc = (int)val;
-        else if (is("mx_digits") && val >= 0 && val <= 2) g_tune.mx_digits = (int)val;
         else return FEATHER_ERR_BAD_ARG;
         p = end;
     }
@@ -876,10 +874,10 @@ static int mx_encode_launch(const void* src, unsigned char* codes, unsigned char
         mx_encode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
             src, reinterpret_cast<uint32_t*>(codes), scales, words);
     } else {
-        const int blocks = mx_blocks(cols);
-        mx_encode_ragged_kernel<T><<<stream_grid(rows * blocks, dev), 256, 0, s>>>(
+        const int blocks = mx_blocks(cols), runs = (blocks + kMxRun - 1) / kMxRun;
+        mx_encode_ragged_kernel<T><<<stream_grid(rows * runs, dev), 256, 0, s>>>(
             reinterpret_cast<const typename MxElem<T>::type*>(src), reinterpret_cast<uint32_t*>(codes), scales, rows,
-            cols, blocks);
+            cols, blocks, runs);
     }
     return launch_status();
 }
@@ -892,27 +890,27 @@ static int mx_decode_launch(const unsigned char* codes, const unsigned char* sca
         mx_decode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
             reinterpret_cast<const uint32_t*>(codes), scales, dst, words);
     } else {
-        const int blocks = mx_blocks(cols);
-        mx_decode_ragged_kernel<T><<<stream_grid(rows * blocks, dev), 256, 0, s>>>(
-            codes, scales, reinterpret_cast<typename MxElem<T>::type*>(dst), rows, cols, blocks);
+        const int blocks = mx_blocks(cols), runs = (blocks + kMxRun - 1) / kMxRun;
+        mx_decode_ragged_kernel<T><<<stream_grid(rows * runs, dev), 256, 0, s>>>(
+            codes, scales, reinterpret_cast<typename MxElem<T>::type*>(dst), rows, cols, blocks, runs);
     }
     return launch_status();
 }
 
-template <int COLS, int ROWS, int STEP, typename K>
-static int mx_gemv_launch(K kernel, MxGemvArgs a, std::atomic<unsigned long long>& configured, const DeviceInfo& dev,
-                          cudaStream_t s) {
-    // ROWS: rows of a task, STEP: blocks of a row a warp takes at a time
-    constexpr int kMostBlocks = (kMgVecHalfs / COLS / kMxBlock) & ~7;
-    a.chunk_blocks = a.blocks < kMostBlocks ? (a.blocks + 7) & ~7 : kMostBlocks;
+template <int VT, int COLS>
+static int mx_gemv_many(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
+    auto kernel = mx_gemv_many_kernel<VT, COLS, 1>;
+    constexpr int kMostBlocks = (kMgVecHalfs / COLS / kMxBlock) & ~3;
+    a.chunk_blocks = a.blocks < kMostBlocks ? (a.blocks + 3) & ~3 : kMostBlocks;
+    static std::atomic<unsigned long long> configured{0};
     if (int st = ensure_smem(kernel, mg_smem_bytes(COLS, kMostBlocks, COLS, kMgPartFloats), configured)) return st;
-    const int steps = ((a.blocks < a.chunk_blocks ? a.blocks : a.chunk_blocks) + STEP - 1) / STEP;
+    const int tiles = ((a.blocks < a.chunk_blocks ? a.blocks : a.chunk_blocks) + 3) / 4;
     a.col_warps = kMgWarps;
-    while (a.col_warps > 1 && a.col_warps > steps) a.col_warps >>= 1;
-    a.slots = kMgPartFloats / (a.col_warps * a.nv * ROWS);
-    const long long units = STEP == 8 ? (a.M + 7) / 8 : (a.M + 15) / 16;
+    while (a.col_warps > 1 && a.col_warps > tiles) a.col_warps >>= 1;
+    a.slots = kMgPartFloats / (a.col_warps * a.nv * 16);
+    const long long groups = (a.M + 15) / 16;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units < dev.sm_count ? units : dev.sm_count));
+    cfg.gridDim = dim3((unsigned)(groups < dev.sm_count ? groups : dev.sm_count));
     cfg.blockDim = dim3(kMgThreads);
     cfg.dynamicSmemBytes = mg_smem_bytes(COLS, a.chunk_blocks, a.nv, kMgPartFloats);
     cfg.stream = s;
@@ -922,12 +920,6 @@ static int mx_gemv_launch(K kernel, MxGemvArgs a, std::atomic<unsigned long long
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
-}
-
-template <int VT, int COLS, int R, bool WIDE>
-static int mx_gemv_line(const MxGemvArgs& a, const DeviceInfo& dev, cudaStream_t s) {
-    static std::atomic<unsigned long long> configured{0};
-    return mx_gemv_launch<COLS, 8 * R, 8>(mx_gemv_line_kernel<VT, COLS, R, WIDE>, a, configured, dev, s);
 }
 
 // kMgWarps x SLOTS x 4 KB of codes in flight, the vector chunk and partial sums in what is left.
@@ -951,8 +943,11 @@ static int mx_gemv_ring(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
     if (!(WHOLE ? mr_make_map(&map, a.codes, 16ll * a.blocks, a.M) : atc_make_map(&map, a.codes, 16 * a.blocks, a.M, 128, kMrRows, true)))
         return FEATHER_ERR_LAUNCH;
     const long long groups = (a.M + kMrRows - 1) / kMrRows;
+    const int grid = (int)(groups < dev.sm_count ? groups : dev.sm_count);
+    a.groups_each = (int)(groups / grid);
+    a.groups_more = (int)(groups % grid);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(groups < dev.sm_count ? groups : dev.sm_count));
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kMgThreads);
     cfg.dynamicSmemBytes = kRing + kBars + mg_smem_bytes(COLS, a.chunk_blocks, a.nv, kMrPartFloats);
     cfg.stream = s;
@@ -966,18 +961,11 @@ static int mx_gemv_ring(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
 
 template <int VT, int COLS>
 static int mx_gemv_cols(const MxGemvArgs& a, const DeviceInfo& dev, cudaStream_t s) {
-    if constexpr (COLS <= 2) {
-        if (a.M * a.blocks >= 128ll * dev.sm_count * (kMrSlotBytes / 16))
-            return a.blocks % 8 == 0 && aligned(a.scales, 2) ? mx_gemv_ring<VT, COLS, 2, true>(a, dev, s)
-                                                            : mx_gemv_ring<VT, COLS, 2, false>(a, dev, s);
-        const bool wide = a.blocks % 2 == 0 && aligned(a.codes, 32) && aligned(a.scales, 2);
-        const bool many = (a.M + 7) / 8 > dev.sm_count;   // two groups of rows at once where a CTA has them
-        return many ? (wide ? mx_gemv_line<VT, COLS, 2, true>(a, dev, s) : mx_gemv_line<VT, COLS, 2, false>(a, dev, s))
-                    : (wide ? mx_gemv_line<VT, COLS, 1, true>(a, dev, s) : mx_gemv_line<VT, COLS, 1, false>(a, dev, s));
-    } else {
-        static std::atomic<unsigned long long> configured{0};
-        return mx_gemv_launch<COLS, 16, 4>(mx_gemv_many_kernel<VT, COLS, 1>, a, configured, dev, s);
-    }
+    if constexpr (COLS <= 2)
+        return a.blocks % 8 == 0 && aligned(a.scales, 2) ? mx_gemv_ring<VT, COLS, 2, true>(a, dev, s)
+                                                        : mx_gemv_ring<VT, COLS, 2, false>(a, dev, s);
+    else
+        return mx_gemv_many<VT, COLS>(a, dev, s);
 }
 
 template <int VT>
@@ -1047,11 +1035,12 @@ static int mx_scale_align(const void* m_scales, const void* x_scales, int blocks
                                                                               : 1;
 }
 
-// Which vectors go through the product kernel.
+// Which dense vectors go through the product kernel as digits: three columns of the GEMV kernels
+// or more, times the matrix.  Measured (us, many-column GEMV against digits): 8192^2 x 3 FP16 22.4 / 14.6,
+// 4096^2 x 8 14.8 / 12.1, x 3 9.4 / 10.2, 2048^2 x 8 6.7 / 9.0, 256 x 2048 x 8 6.6 / 9.0.
 static bool mx_wants_digits(long long M, long long N, int batch, int v_dtype) {
-    const int knob = g_tune.mx_digits.load(std::memory_order_relaxed);
-    (void)batch; (void)v_dtype;
-    return knob == 2 || (knob == 1 && M * N >= (8ll << 20));
+    const long long cols = (long long)batch * (v_dtype == FEATHER_SRC_F32 ? 2 : 1);
+    return cols > 2 && cols * M * N >= (80ll << 20);
 }
 
 // Tiles of 224 or of 128 rows of x: those whose waves take less, a wave of the wide ones taking
@@ -1115,13 +1104,21 @@ static int mx_gemv_digits(const MxGemvArgs& v, int batch, unsigned char* workspa
 }
 
 template <int T, int MODE>
-static int rotary_launch(const RotaryArgs& a, const DeviceInfo& dev, cudaStream_t s) {
-    constexpr int V = T == kSrcF32 ? 4 : 8;
-    const bool wide = aligned(a.x, 16) && aligned(a.out, MODE < 0 ? 16 : V) && (a.rotated / 2) % V == 0 && a.dim % V == 0 &&
-                      a.token_stride % V == 0 && a.head_stride % V == 0;
-    const long long most = 16ll * dev.sm_count;
-    const unsigned grid = (unsigned)(a.tokens < most ? a.tokens : most);
-    if (wide) rotary_kernel<T, MODE, V><<<grid, kRotThreads, 0, s>>>(a);
+static int rotary_launch(RotaryArgs a, const DeviceInfo& dev, cudaStream_t s) {
+    constexpr int kWide = T == kSrcF32 ? 4 : 8;
+    const bool wide = aligned(a.x, 16) && aligned(a.out, MODE < 0 ? 16 : kWide) && (a.rotated / 2) % kWide == 0 &&
+                      a.dim % kWide == 0 && a.token_stride % kWide == 0 && a.head_stride % kWide == 0;
+    const int v = wide ? kWide : 1;
+    const long long items = (long long)a.heads * (a.rotated / 2 / v + (a.dim - a.rotated + 2 * v - 1) / (2 * v));
+    // eight CTAs per SM walk the tokens; few tokens share their heads out among more CTAs
+    const long long most = 8ll * dev.sm_count, rounds = (items + kRotThreads - 1) / kRotThreads;
+    const long long gx = a.tokens < most ? a.tokens : most;
+    long long gy = most / gx < rounds ? most / gx : rounds;
+    const long long per = (rounds + gy - 1) / gy * kRotThreads;
+    gy = (items + per - 1) / per;
+    a.items_each = (int)per;
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (wide) rotary_kernel<T, MODE, kWide><<<grid, kRotThreads, 0, s>>>(a);
     else rotary_kernel<T, MODE, 1><<<grid, kRotThreads, 0, s>>>(a);
     return launch_status();
 }
@@ -1778,7 +1775,7 @@ int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const vo
                : v_dtype == FEATHER_SRC_F32 ? mx_gemv_digits<kSrcF32>(a, batch, w, *dev, s)
                                             : mx_gemv_digits<kSrcBF16>(a, batch, w, *dev, s);
     }
-    if (packed && mx_wants_digits(M, N, batch, v_dtype)) {
+    if (packed && batch > 1) {
         MxGemmArgs x = {};
         x.m_codes = m_codes;
         x.m_scales = m_scales;

@@ -154,27 +154,38 @@ mx_encode_kernel(const void* __restrict__ src, uint32_t* __restrict__ codes, uns
     }
 }
 
-// Any row length and alignment: a warp per block, one element per lane (consecutive loads
-// whatever the row's start), the maximum with one warp reduction.
+// Any row length and alignment: a warp takes kMxRun consecutive blocks of a row, one element of
+// each per lane (consecutive loads whatever the row's start), the maximum with one warp reduction.
+constexpr int kMxRun = 8;
 template <int T>
 __global__ void __launch_bounds__(256)
 mx_encode_ragged_kernel(const typename MxElem<T>::type* __restrict__ src, uint32_t* __restrict__ codes,
-                        unsigned char* __restrict__ scales, long long rows, long long cols, int blocks_row) {
+                        unsigned char* __restrict__ scales, long long rows, long long cols, int blocks_row, int runs_row) {
     const int lane = threadIdx.x & 31;
-    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
-    const long long n_blocks = rows * blocks_row;
-    for (long long blk = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; blk < n_blocks; blk += warps) {
-        const long long row = blk / blocks_row;
-        const long long col = (blk - row * blocks_row) * kMxBlock + lane;
-        const float x = col < cols ? MxElem<T>::get(src[row * cols + col]) : 0.f;
-        const uint32_t b = mx_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(x) & 0x7FFFFFFFu));
-        const float y[8] = {x * mx_to_grid(b), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t c = (b == 255u ? 0u : mx_encode8(y) & 0xFu) << (4 * (lane & 7));
-        c |= __shfl_xor_sync(0xFFFFFFFFu, c, 1);
-        c |= __shfl_xor_sync(0xFFFFFFFFu, c, 2);
-        c |= __shfl_xor_sync(0xFFFFFFFFu, c, 4);
-        if ((lane & 7) == 0) codes[blk * 4 + (lane >> 3)] = c;
-        if (lane == 0) scales[blk] = (unsigned char)b;
+    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, runs = rows * runs_row;
+    for (long long run = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; run < runs; run += warps) {
+        const long long row = runs >> 32 ? run / runs_row : (uint32_t)run / (uint32_t)runs_row;
+        const int b0 = (int)(run - row * runs_row) * kMxRun;
+        const typename MxElem<T>::type* from = src + row * cols;
+        float x[kMxRun];
+#pragma unroll
+        for (int u = 0; u < kMxRun; ++u) {
+            const long long col = (long long)(b0 + u) * kMxBlock + lane;
+            x[u] = col < cols ? MxElem<T>::get(from[col]) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kMxRun; ++u) {
+            if (b0 + u >= blocks_row) break;
+            const uint32_t b = mx_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(x[u]) & 0x7FFFFFFFu));
+            const float y[8] = {x[u] * mx_to_grid(b), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            uint32_t c = (b == 255u ? 0u : mx_encode8(y) & 0xFu) << (4 * (lane & 7));
+            c |= __shfl_xor_sync(0xFFFFFFFFu, c, 1);
+            c |= __shfl_xor_sync(0xFFFFFFFFu, c, 2);
+            c |= __shfl_xor_sync(0xFFFFFFFFu, c, 4);
+            const long long blk = row * blocks_row + b0 + u;
+            if ((lane & 7) == 0) codes[blk * 4 + (lane >> 3)] = c;
+            if (lane == 0) scales[blk] = (unsigned char)b;
+        }
     }
 }
 
@@ -236,21 +247,33 @@ mx_decode_kernel(const uint32_t* __restrict__ codes, const unsigned char* __rest
     }
 }
 
-// Any row length and alignment: consecutive lanes take consecutive elements of a row.
+// Any row length and alignment: a warp takes kMxRun consecutive blocks of a row, consecutive lanes
+// consecutive elements.
 template <int T>
 __global__ void __launch_bounds__(256)
 mx_decode_ragged_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                        typename MxElem<T>::type* __restrict__ dst, long long rows, long long cols, int blocks_row) {
+                        typename MxElem<T>::type* __restrict__ dst, long long rows, long long cols, int blocks_row,
+                        int runs_row) {
     const int lane = threadIdx.x & 31;
-    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
-    const long long n_blocks = rows * blocks_row;
-    for (long long blk = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; blk < n_blocks; blk += warps) {
-        const long long row = blk / blocks_row;
-        const long long col = (blk - row * blocks_row) * kMxBlock + lane;
-        const uint32_t pair = codes[blk * 16 + (lane >> 1)];
-        uint32_t h[4];
-        mx_decode8(lane & 1 ? pair >> 4 : pair, h);
-        if (col < cols) dst[row * cols + col] = MxElem<T>::put(h2_to_f2(h[0]).x * mx_scale_value(scales[blk]));
+    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, runs = rows * runs_row;
+    for (long long run = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; run < runs; run += warps) {
+        const long long row = runs >> 32 ? run / runs_row : (uint32_t)run / (uint32_t)runs_row;
+        const int b0 = (int)(run - row * runs_row) * kMxRun;
+        const long long blk = row * blocks_row + b0;
+        uint32_t pair[kMxRun], s[kMxRun];
+#pragma unroll
+        for (int u = 0; u < kMxRun; ++u) {
+            const bool there = b0 + u < blocks_row;
+            pair[u] = there ? codes[(blk + u) * 16 + (lane >> 1)] : 0u;
+            s[u] = there ? scales[blk + u] : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kMxRun; ++u) {
+            const long long col = (long long)(b0 + u) * kMxBlock + lane;
+            uint32_t h[4];
+            mx_decode8(lane & 1 ? pair[u] >> 4 : pair[u], h);
+            if (col < cols) dst[row * cols + col] = MxElem<T>::put(h2_to_f2(h[0]).x * mx_scale_value(s[u]));
+        }
     }
 }
 

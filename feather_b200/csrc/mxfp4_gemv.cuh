@@ -58,13 +58,6 @@ __device__ __forceinline__ float2 mx_scale_pair(uint32_t s) {
     return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xFFFF0000u));
 }
 
-// 32 bytes, 32-byte aligned.
-__device__ __forceinline__ void ldg_line(const uint4* p, uint32_t (&r)[8]) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "l"(p));
-}
-
 struct MxGemvArgs {
     const unsigned char* codes;
     const unsigned char* scales;
@@ -77,8 +70,9 @@ struct MxGemvArgs {
     int chunk_blocks;                // blocks of the vector in shared memory at a time, a multiple of 8
     int slots;                       // tasks whose partial sums fit
     int part_floats;                 // room for partial sums
+    int groups_each, groups_more;    // row groups of every CTA, and CTAs with one more
     unsigned int* status;
-    int col_warps;                   // warps that split a row's columns: a power of two, at most the first chunk's tiles or lines
+    int col_warps;                   // warps that split a row's columns: a power of two, at most the first chunk's tiles or spans
 };
 
 // Layout of dynamic shared memory: COLS columns of chunk + 8 halfs, block scales [nv][chunk_blocks],
@@ -89,68 +83,99 @@ __host__ __device__ constexpr int mg_smem_bytes(int cols, int chunk_blocks, int 
 }
 
 // Blocks [blk0, blk0 + pad_blk) of the vectors to shared memory, those from n_blk on as zeros: four
-// threads per block, eight elements each.
-template <int VT>
+// threads per block, eight elements each, the loads of a few such pieces in flight.  `between` runs
+// behind the first loads: what it starts overlaps their latency.
+template <int VT, typename F>
 __device__ __forceinline__ void mg_stage(const MxGemvArgs& a, __half* vec, float* vscale, int column, int blk0, int n_blk,
-                                         int pad_blk, int tid) {
+                                         int pad_blk, int tid, F&& between) {
     constexpr int kParts = VT == kSrcF32 ? 2 : 1;
-    const int warp = tid >> 5, lane = tid & 31;
-                    const int quads = a.nv * pad_blk;
-                    for (int i0 = warp * 32; i0 < quads * 4; i0 += kMgThreads) {   // whole warps: the lanes shuffle
-                        const int i = i0 + lane, q = i & 3, b = (i >> 2) % pad_blk;
-                        const bool mine = (i >> 2) < quads;
-                        const int n = mine ? (i >> 2) / pad_blk : 0;
-                        const long long e0 = (long long)(blk0 + b) * kMxBlock + q * 8;
-                        float x[8];
-                        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-                        float sv = 1.f;
-                        if constexpr (VT == kSrcMxfp4) {
-                            if (b < n_blk) {
-                                const long long at = (long long)n * a.blocks + blk0 + b;
-                                mx_decode8(__ldg(reinterpret_cast<const uint32_t*>(a.v) + at * 4 + q), hi);
-                                sv = mx_scale_value(__ldg(a.v_scales + at));
-                            }
-                        } else {
-                            typedef typename MxElem<VT>::type E;
-                            const E* p = reinterpret_cast<const E*>(a.v) + (long long)n * a.N + e0;
-                            uint32_t top = 0u;
-                            if (e0 + 8 <= a.N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-                                mx_load8<VT>(p, 0, x);
-                            } else {
-    #pragma unroll
-                                for (int k = 0; k < 8; ++k) x[k] = e0 + k < a.N ? MxElem<VT>::get(p[k]) : 0.f;
-                            }
-    #pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                const uint32_t u = __float_as_uint(x[k]) & 0x7FFFFFFFu;
-                                if (u < 0x7F800000u) top = max(top, u);
-                            }
-                            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                            const uint32_t f = min(268u - (top >> 23), 253u);   // exponent field of the factor
-                            const float factor = __uint_as_float(f << 23);
-                            sv = __uint_as_float((254u - f) << 23);
-    #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                float y[2], z[2];
-                                unsigned short w[2], l[2];
-    #pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-                                    y[j] = x[2 * k + j] * factor;
-                                    w[j] = __half_as_ushort(__float2half_rn(y[j]));
-                                    z[j] = y[j] - __half2float(__ushort_as_half(w[j]));
-                                    l[j] = (w[j] & 0x7C00u) == 0x7C00u ? 0 : __half_as_ushort(__float2half_rn(z[j]));
-                                }
-                                hi[k] = w[0] | ((uint32_t)w[1] << 16);
-                                lo[k] = l[0] | ((uint32_t)l[1] << 16);
-                            }
-                        }
-                        if (!mine) continue;
-                        __half* d = vec + (long long)n * kParts * column + b * kMxBlock + q * 8;
-                        *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        if (kParts == 2) *reinterpret_cast<uint4*>(d + column) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        if (q == 0) vscale[n * a.chunk_blocks + b] = sv;
+    constexpr int kWords = VT == kSrcF32 ? 8 : VT == kSrcMxfp4 ? 1 : 4;   // of eight elements
+    constexpr int kBatch = VT == kSrcF32 ? 2 : 4, kStep = kMgThreads / 4;
+    const int q = tid & 3, pieces = a.nv * pad_blk;
+    bool begun = false;
+    for (int base = 0; base < pieces; base += kBatch * kStep) {
+        uint32_t raw[kBatch][kWords];
+        uint32_t sb[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (base + u * kStep >= pieces) break;           // the same for every thread
+            const int i = min(base + u * kStep + (tid >> 2), pieces - 1), n = i / pad_blk, b = i - n * pad_blk;
+            const long long e0 = (long long)(blk0 + b) * kMxBlock + q * 8;
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) raw[u][k] = 0u;
+            sb[u] = 127u;
+            if (b >= n_blk) continue;
+            if constexpr (VT == kSrcMxfp4) {
+                const long long at = (long long)n * a.blocks + blk0 + b;
+                raw[u][0] = __ldg(reinterpret_cast<const uint32_t*>(a.v) + at * 4 + q);
+                sb[u] = __ldg(a.v_scales + at);
+            } else {
+                typedef typename MxElem<VT>::type E;
+                const E* p = reinterpret_cast<const E*>(a.v) + (long long)n * a.N + e0;
+                if (e0 + 8 <= a.N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+                    for (int k = 0; k < kWords / 4; ++k) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + k);
+                        raw[u][4 * k] = x.x; raw[u][4 * k + 1] = x.y; raw[u][4 * k + 2] = x.z; raw[u][4 * k + 3] = x.w;
                     }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (e0 + k >= a.N) continue;
+                        if constexpr (VT == kSrcF32) raw[u][k] = __float_as_uint(p[k]);
+                        else raw[u][k / 2] |= (uint32_t)p[k] << (16 * (k & 1));
+                    }
+                }
+            }
+        }
+        if (!begun) between();
+        begun = true;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (base + u * kStep >= pieces) break;
+            const int i = base + u * kStep + (tid >> 2), n = min(i, pieces - 1) / pad_blk, b = min(i, pieces - 1) - n * pad_blk;
+            uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+            float sv;
+            if constexpr (VT == kSrcMxfp4) {
+                mx_decode8(raw[u][0], hi);
+                sv = mx_scale_value(sb[u]);
+            } else {
+                float x[8];
+                uint32_t top = 0u;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (VT == kSrcF32) x[k] = __uint_as_float(raw[u][k]);
+                    else x[k] = MxElem<VT>::get((unsigned short)(raw[u][k / 2] >> (16 * (k & 1))));
+                    const uint32_t m = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+                    if (m < 0x7F800000u) top = max(top, m);
+                }
+                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                const uint32_t f = min(268u - (top >> 23), 253u);   // exponent field of the factor
+                const float factor = __uint_as_float(f << 23);
+                sv = __uint_as_float((254u - f) << 23);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    unsigned short h[2], l[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float y = x[2 * k + j] * factor;
+                        h[j] = __half_as_ushort(__float2half_rn(y));
+                        const float z = y - __half2float(__ushort_as_half(h[j]));
+                        l[j] = (h[j] & 0x7C00u) == 0x7C00u ? 0 : __half_as_ushort(__float2half_rn(z));
+                    }
+                    hi[k] = h[0] | ((uint32_t)h[1] << 16);
+                    lo[k] = l[0] | ((uint32_t)l[1] << 16);
+                }
+            }
+            if (i < pieces) {
+                __half* d = vec + (long long)n * kParts * column + b * kMxBlock + q * 8;
+                *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (kParts == 2) *reinterpret_cast<uint4*>(d + column) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                if (q == 0) vscale[n * a.chunk_blocks + b] = sv;
+            }
+        }
+    }
 }
 
 // VT: type of the vector (kSrc...); COLS: columns, 1, 2, 4 or 8 (an FP32 vector takes two); R:
@@ -228,7 +253,7 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
             // the vector chunk: four threads per block, eight elements each
             if (ch > 0 || first > 0 ? chunks > 1 : true) {
                 if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
-                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, tiles * 4, tid);
+                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, tiles * 4, tid, [] {});
                 __syncthreads();
             }
 
@@ -341,185 +366,19 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
     }
 }
 
-// One or two columns (a vector, an FP32 vector in two parts, two vectors).  A lane takes 32 bytes of
-// a row, two neighbouring blocks, and the four lanes of a row a whole 128-byte line: half the lines
-// per load instruction.  The product's rows 0-7 are the first blocks of eight rows, its rows 8-15
-// the second blocks of the same rows; column n holds the vector for block n of the line, zero but
-// in the slots of lane n / 2.  Of the four sums a lane gets back, the first is its first block's and
-// the last its second block's.  WIDE: 32-byte loads (rows of an even number of blocks).
-template <int VT, int COLS, int R, bool WIDE>
-__global__ void __launch_bounds__(kMgThreads, 1)
-mx_gemv_line_kernel(const MxGemvArgs a) {
-    constexpr int kParts = VT == kSrcF32 ? 2 : 1;
-    constexpr int kAcc = COLS / kParts;
-    constexpr int kBuf = R == 1 ? 6 : 4;
-    extern __shared__ __align__(16) unsigned char mg_smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int column = mg_column(a.chunk_blocks);
-    __half* vec = reinterpret_cast<__half*>(mg_smem);
-    float* vscale = reinterpret_cast<float*>(mg_smem + COLS * column * 2);
-    unsigned char* zeros = mg_smem + COLS * column * 2 + 4 * a.nv * a.chunk_blocks;
-    float* part = reinterpret_cast<float*>(zeros + 64);
-
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-
-    const long long groups = (a.M + 7) / 8;
-    const long long g_begin = groups * blockIdx.x / gridDim.x, g_end = groups * (blockIdx.x + 1) / gridDim.x;
-    const int my_groups = (int)(g_end - g_begin);
-    const int tasks = (my_groups + R - 1) / R;
-    const int my_rows = (int)min(a.M - g_begin * 8, (long long)my_groups * 8);
-    const uint4* codes = reinterpret_cast<const uint4*>(a.codes) + g_begin * 8 * a.blocks;
-    const unsigned char* scales = a.scales + g_begin * 8 * a.blocks;
-    if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0u;
-
-    const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
-    const int wk = a.col_warps, wr = kMgWarps / wk, my_k = warp & (wk - 1), my_r = warp / wk;
-    for (int first = 0; first < tasks; first += a.slots) {
-        const int n_tasks = min(a.slots, tasks - first);
-        for (int ch = 0; ch < chunks; ++ch) {
-            const int blk0 = ch * a.chunk_blocks, n_blk = min(a.chunk_blocks, a.blocks - blk0);
-            const int lines = (n_blk + 7) / 8;
-            const int line_begin = lines * my_k / wk, my_lines = lines * (my_k + 1) / wk - line_begin;
-            const int my_tasks = my_r < n_tasks ? (n_tasks - my_r + wr - 1) / wr : 0;
-            const int steps = my_tasks * my_lines;
-
-            // The matrix loads, along this warp's walk (its tasks, inside them its lines).  Offsets
-            // count from the CTA's first row in 32 bits.  Rows past the last are the last row again
-            // and blocks past the row's end its last blocks again: the former are not stored, the
-            // latter meet a vector of zeros.
-            uint32_t m[kBuf][R][8];
-            uint32_t s[kBuf][R];
-            uint32_t row_at[R];
-            int l_line = 0, l_task = my_r;
-            auto load = [&](int buf) {
-                if (l_line == 0) {
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        row_at[r] = (uint32_t)min(((first + l_task) * R + r) * 8 + g, my_rows - 1) * (uint32_t)a.blocks;
-                }
-                const int blk = (line_begin + l_line) * 8 + 2 * t;
-                const uint32_t b0 = (uint32_t)(blk0 + min(blk, WIDE ? n_blk - 2 : n_blk - 1));
-                const uint32_t b1 = (uint32_t)(blk0 + min(blk + 1, n_blk - 1));
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    if constexpr (WIDE) {
-                        ldg_line(codes + row_at[r] + b0, m[buf][r]);
-                        s[buf][r] = __ldg(reinterpret_cast<const unsigned short*>(scales + row_at[r] + b0));
-                    } else {
-                        const uint4 x = ldg_stream(codes + row_at[r] + b0), y = ldg_stream(codes + row_at[r] + b1);
-                        m[buf][r][0] = x.x; m[buf][r][1] = x.y; m[buf][r][2] = x.z; m[buf][r][3] = x.w;
-                        m[buf][r][4] = y.x; m[buf][r][5] = y.y; m[buf][r][6] = y.z; m[buf][r][7] = y.w;
-                        s[buf][r] = __ldg(scales + row_at[r] + b0) | ((uint32_t)__ldg(scales + row_at[r] + b1) << 8);
-                    }
-                }
-                if (++l_line == my_lines) l_line = 0, l_task += wr;
-            };
-#pragma unroll
-            for (int i = 0; i < kBuf - 1; ++i)
-                if (i < steps) load(i);
-
-            if (ch > 0 || first > 0 ? chunks > 1 : true) {
-                if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
-                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, lines * 8, tid);
-                __syncthreads();
-            }
-
-            float acc[R][kAcc];
-            int line = 0, task = my_r;
-            const bool diag = (g >> 1) == t;        // this lane's column is of one of its own blocks
-            auto multiply = [&](int buf) {
-                if (line == 0) {
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int n = 0; n < kAcc; ++n) acc[r][n] = 0.f;
-                }
-                const int b = (line_begin + line) * 8;      // the line's first block inside the chunk
-                const uint4* src[COLS];
-                float c[R][COLS][4];
-#pragma unroll
-                for (int p = 0; p < COLS; ++p) {
-                    src[p] = reinterpret_cast<const uint4*>(
-                        diag ? reinterpret_cast<const unsigned char*>(vec + p * column + (b + g) * kMxBlock) : zeros);
-#pragma unroll
-                    for (int r = 0; r < R; ++r) c[r][p][0] = c[r][p][1] = c[r][p][2] = c[r][p][3] = 0.f;
-                }
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint4 bv[COLS];
-#pragma unroll
-                    for (int p = 0; p < COLS; ++p) bv[p] = src[p][w];
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        uint32_t x[4], y[4];
-                        mx_decode8(m[buf][r][w], x);
-                        mx_decode8(m[buf][r][4 + w], y);
-#pragma unroll
-                        for (int p = 0; p < COLS; ++p) {
-                            mma_f16(c[r][p], x[0], y[0], x[1], y[1], bv[p].x, bv[p].y);
-                            mma_f16(c[r][p], x[2], y[2], x[3], y[3], bv[p].z, bv[p].w);
-                        }
-                    }
-                }
-                // (a block's sum) x (the vector block's power of two) x (the matrix block's)
-#pragma unroll
-                for (int n = 0; n < kAcc; ++n) {
-                    const float2 sv = *reinterpret_cast<const float2*>(vscale + n * a.chunk_blocks + b + 2 * t);
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const float2 sw = mx_scale_pair(s[buf][r]);
-                        const float c0 = kParts == 2 ? c[r][0][0] + c[r][COLS - 1][0] : c[r][n][0];
-                        const float c1 = kParts == 2 ? c[r][0][3] + c[r][COLS - 1][3] : c[r][n][3];
-                        acc[r][n] = fmaf(c0 * sv.x, sw.x, acc[r][n]);
-                        acc[r][n] = fmaf(c1 * sv.y, sw.y, acc[r][n]);
-                    }
-                }
-                if (++line == my_lines) {
-                    // the row's partial sums: over the four lanes, then one slot per warp
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int n = 0; n < kAcc; ++n) {
-                            float x = acc[r][n];
-                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
-                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
-                            if (t == 0) {
-                                float* to = part + ((task * wk + my_k) * kAcc + n) * (8 * R) + r * 8 + g;
-                                *to = ch == 0 ? x : *to + x;
-                            }
-                        }
-                    line = 0;
-                    task += wr;
-                }
-            };
-            for (int i = 0; i < steps; i += kBuf) {
-#pragma unroll
-                for (int u = 0; u < kBuf; ++u) {
-                    if (i + u < steps) {
-                        if (i + u + kBuf - 1 < steps) load((u + kBuf - 1) % kBuf);
-                        multiply(u);
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        for (int i = tid; i < n_tasks * kAcc * 8 * R; i += kMgThreads) {
-            const int r = i % (8 * R), n = (i / (8 * R)) % kAcc, task = i / (8 * R * kAcc);
-            const int row = (first + task) * R * 8 + r;
-            float x = 0.f;
-            for (int k = 0; k < wk; ++k) x += part[((task * wk + k) * kAcc + n) * (8 * R) + r];
-            if (row < my_rows) a.out[n * a.M + g_begin * 8 + row] = x;
-        }
-        __syncthreads();
-    }
-}
-
-// Large matrices: the line kernel's arithmetic with the codes coming through shared memory.  A warp
-// owns kMrSlots slots of 4 KB, 16 rows x 512 codes (two lines), that it fills itself with
-// tensor-map copies (128-byte swizzle: the reads below are free of bank conflicts); it refills a
-// slot as soon as it has read it, so nothing is shared and nothing but arrival is waited for.
-// Loads to registers (the line kernel) keep far fewer bytes in flight than their count suggests.
+// One or two columns (a vector, an FP32 vector in two parts, two vectors), any size.
+//
+// A lane takes 32 bytes of a row, two neighbouring blocks, and the four lanes of a row a whole
+// 128-byte line.  The product's rows 0-7 are the first blocks of eight rows, its rows 8-15 the
+// second blocks of the same rows; column n holds the vector for block n of the line, zero but
+// in the slots of lane n / 2.  Of the four sums a lane gets back, the first is its first block's
+// and the last its second block's.
+//
+// The codes come through shared memory.  A warp owns SLOTS slots of 4 KB, 16 rows x 512 codes (two
+// lines), that it fills itself with tensor-map copies (128-byte swizzle: the reads below are free of
+// bank conflicts); it refills a slot as soon as it has read it, so nothing is shared and nothing
+// but arrival is waited for.  Loads straight to registers reached 3.9 TB/s at 16384 x 16384 (the
+// bytes in flight hang on the scoreboard), this 5.0.
 constexpr int kMrRows = 16, kMrLines = 2, kMrSlotBytes = kMrRows * kMrLines * 128;
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -567,17 +426,17 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
         for (int i = 0; i < SLOTS; ++i) mbar_init(bars + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncwarp();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-
-    const long long groups = (a.M + kMrRows - 1) / kMrRows;
-    const int g_begin = (int)(groups * blockIdx.x / gridDim.x), tasks = (int)(groups * (blockIdx.x + 1) / gridDim.x) - g_begin;
+    // everything that needs no memory is behind us when the kernel before this one has ended
+    const int extra = min((int)blockIdx.x, a.groups_more);
+    const int g_begin = (int)blockIdx.x * a.groups_each + extra, tasks = a.groups_each + ((int)blockIdx.x < a.groups_more ? 1 : 0);
     const int my_rows = (int)min(a.M - (long long)g_begin * kMrRows, (long long)tasks * kMrRows);
     const unsigned char* scales = a.scales + (long long)g_begin * kMrRows * a.blocks;
     if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0u;
 
     const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
     const int wk = a.col_warps, wr = kMgWarps / wk, my_k = warp & (wk - 1), my_r = warp / wk;
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     bool ok = true;
     int used = 0;                                    // slots filled so far, over all chunks
     for (int first = 0; first < tasks; first += a.slots) {
@@ -604,8 +463,9 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
                 }
                 if (++l_span == my_spans) l_span = 0, l_task += wr;
             };
-            for (int i = 0; i < SLOTS && i < steps; ++i) fill((used + i) % SLOTS);
-
+            auto begin = [&] {
+                for (int i = 0; i < SLOTS && i < steps; ++i) fill((used + i) % SLOTS);
+            };
             // scale bytes of a step, two blocks of two lines of R rows, a step ahead
             uint32_t s[kMrLines][R], s_next[kMrLines][R];
             int s_span = 0, s_task = my_r;
@@ -627,12 +487,14 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
                 }
                 if (++s_span == my_spans) s_span = 0, s_task += wr;
             };
-            if (steps > 0) load_scales();
-
             if (ch > 0 || first > 0 ? chunks > 1 : true) {
                 if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
-                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, spans * 8 * kMrLines, tid);
+                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, spans * 8 * kMrLines, tid, begin);
+                if (steps > 0) load_scales();
                 __syncthreads();
+            } else {
+                begin();
+                if (steps > 0) load_scales();
             }
 
             float acc[R][kAcc];

@@ -85,22 +85,25 @@ struct RotaryArgs {
     void* out;
     long long tokens, token_stride, head_stride;   // strides of x in elements
     int heads, dim, rotated, wide_positions, interleaved;
+    int items_each;             // items of a token per CTA
     float scale;
 };
 
-// A CTA takes a token at a time: angles first, then items of two V-element vectors (a pair of
-// vectors that turn into each other, or 2 V elements that pass through); V = 16 bytes of the
-// input type where sizes, strides and addresses allow, else 1.
+// A CTA takes a token (blockIdx.x + k gridDim.x) and a share of its heads (blockIdx.y) at a time, in
+// items of two V-element vectors: a pair of vectors that turn into each other, or 2 V elements
+// that pass through; V = 16 bytes of the input type where sizes, strides and addresses allow, else
+// 1.  The next token's angles are computed and its first items loaded while this one's items turn.
 template <int T, int MODE, int V>
 __global__ void __launch_bounds__(kRotThreads)
 rotary_kernel(const RotaryArgs a) {
     typedef typename MxElem<T>::type E;
-    __shared__ float2 turn[kRotMaxPairs];
+    __shared__ float2 turns[2][kRotMaxPairs];
     const int half = a.rotated / 2;
-    const int turned = half / V;                             // items of a head that turn
+    const int turned = half / V;                                   // items of a head that turn
     const int still = (a.dim - a.rotated + 2 * V - 1) / (2 * V);   // items that pass through
     const int items = turned + still;
-    for (long long t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int j_begin = (int)blockIdx.y * a.items_each, j_end = min(j_begin + a.items_each, a.heads * items);
+    auto angles = [&](long long t, float2* turn) {
         const double p = a.wide_positions ? (double)reinterpret_cast<const long long*>(a.positions)[t]
                                           : (double)reinterpret_cast<const int*>(a.positions)[t];
         for (int i = threadIdx.x; i < half; i += kRotThreads) {
@@ -109,19 +112,47 @@ rotary_kernel(const RotaryArgs a) {
             cs.y *= a.scale;
             turn[i] = cs;
         }
-        __syncthreads();
-        const E* row = reinterpret_cast<const E*>(a.x) + t * a.token_stride;
-        for (int j = threadIdx.x; j < a.heads * items; j += kRotThreads) {
-            const int h = j / items, k = j - h * items;
-            const E* x = row + h * a.head_stride;
-            const long long o = MODE >= 0 ? ((long long)h * a.tokens + t) * a.dim : (t * a.heads + h) * a.dim;
-            float u[V], v[V];
+    };
+    // an item's place in its head: the two vectors' first elements, and the first pair
+    auto place = [&](int k, int& at_u, int& at_v) {
+        if (k < turned) {
+            at_u = a.interleaved ? 2 * k * V : k * V;
+            at_v = a.interleaved ? at_u + V : at_u + half;
+        } else {
+            at_u = a.rotated + (k - turned) * 2 * V;
+            at_v = at_u + V;
+        }
+    };
+    const int j0 = j_begin + (int)threadIdx.x, h0 = j0 / items, k0 = j0 - h0 * items;   // this thread's first item of every token
+    int u0, v0;
+    place(k0, u0, v0);
+    float u[V], v[V];
+    auto fetch = [&](long long t) {
+        if (j0 >= j_end) return;
+        const E* x = reinterpret_cast<const E*>(a.x) + t * a.token_stride + h0 * a.head_stride;
+        rotary_load<T, V>(x + u0, u);
+        if (v0 < a.dim) rotary_load<T, V>(x + v0, v);
+    };
+    long long t = blockIdx.x;
+    if (t >= a.tokens) return;
+    fetch(t);
+    angles(t, turns[0]);
+    __syncthreads();
+    for (int buf = 0; t < a.tokens; t += gridDim.x, buf ^= 1) {
+        const float2* turn = turns[buf];
+        const bool more = t + gridDim.x < a.tokens;
+        for (int j = j0; j < j_end; j += kRotThreads) {
+            int h = h0, k = k0, at_u = u0, at_v = v0;
+            if (j != j0) {
+                h = j / items;
+                k = j - h * items;
+                place(k, at_u, at_v);
+                const E* x = reinterpret_cast<const E*>(a.x) + t * a.token_stride + h * a.head_stride;
+                rotary_load<T, V>(x + at_u, u);
+                if (at_v < a.dim) rotary_load<T, V>(x + at_v, v);
+            }
             if (k < turned) {
                 const int i = k * V;
-                int at_u = i, at_v = i + half;
-                if (a.interleaved) at_u = 2 * i, at_v = 2 * i + V;
-                rotary_load<T, V>(x + at_u, u);
-                rotary_load<T, V>(x + at_v, v);
                 if (!a.interleaved || V == 1) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
@@ -141,17 +172,14 @@ rotary_kernel(const RotaryArgs a) {
                         v[e + 1] = q0 * c1.y + q1 * c1.x;
                     }
                 }
-                rotary_store<T, MODE, V>(a.out, o + at_u, u);
-                rotary_store<T, MODE, V>(a.out, o + at_v, v);
-            } else {
-                const int i = a.rotated + (k - turned) * 2 * V;
-                rotary_load<T, V>(x + i, u);
-                rotary_store<T, MODE, V>(a.out, o + i, u);
-                if (i + V < a.dim) {
-                    rotary_load<T, V>(x + i + V, v);
-                    rotary_store<T, MODE, V>(a.out, o + i + V, v);
-                }
             }
+            const long long o = MODE >= 0 ? ((long long)h * a.tokens + t) * a.dim : (t * a.heads + h) * a.dim;
+            rotary_store<T, MODE, V>(a.out, o + at_u, u);
+            if (at_v < a.dim) rotary_store<T, MODE, V>(a.out, o + at_v, v);
+        }
+        if (more) {
+            fetch(t + gridDim.x);
+            angles(t + gridDim.x, turns[buf ^ 1]);
         }
         __syncthreads();
     }

@@ -77,7 +77,8 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
         out = torch.empty(batch, M, dtype=torch.float32, device=v.device)
     if M and batch:
         lib = _lib.load()
-        need = lib.feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype) if scales_ptr is None else 0
+        # one FP32 or two 16-bit vectors never need one
+        need = 0 if batch == 1 or scales_ptr is not None else lib.feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype)
         ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
         call(lib.feather_gemv_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr,
                                            out.data_ptr(), ws.data_ptr() if need else None, M, N, batch))
