@@ -1110,10 +1110,15 @@ static int rotary_launch(RotaryArgs a, const DeviceInfo& dev, cudaStream_t s) {
                       a.dim % kWide == 0 && a.token_stride % kWide == 0 && a.head_stride % kWide == 0;
     const int v = wide ? kWide : 1;
     const long long items = (long long)a.heads * (a.rotated / 2 / v + (a.dim - a.rotated + 2 * v - 1) / (2 * v));
-    // eight CTAs per SM walk the tokens; few tokens share their heads out among more CTAs
-    const long long most = 8ll * dev.sm_count, rounds = (items + kRotThreads - 1) / kRotThreads;
-    const long long gx = a.tokens < most ? a.tokens : most;
-    long long gy = most / gx < rounds ? most / gx : rounds;
+    // tiles of up to eight tokens while there are six CTAs per SM; few tokens share their heads out
+    const long long full = 6ll * dev.sm_count, rounds = (items + kRotThreads - 1) / kRotThreads;
+    long long tile = a.tokens / full;
+    tile = tile < 1 ? 1 : tile < kRotTile ? tile : kRotTile;
+    while (tile > 1 && tile * (a.rotated / 2) > kRotAngles) tile /= 2;
+    a.tile = (int)tile;
+    const long long gx = (a.tokens + tile - 1) / tile;
+    if (gx > 0x7FFFFFFFll) return FEATHER_ERR_TOO_LARGE;
+    long long gy = full / gx < 1 ? 1 : full / gx < rounds ? full / gx : rounds;
     const long long per = (rounds + gy - 1) / gy * kRotThreads;
     gy = (items + per - 1) / per;
     a.items_each = (int)per;

@@ -29,9 +29,10 @@ def blocks_of(n: int) -> int:
 
 
 def dtype_id(dtype: torch.dtype, name: str) -> int:
-    if dtype not in DTYPE_IDS:
+    found = DTYPE_IDS.get(dtype)
+    if found is None:
         raise TypeError(f"{name} must be float16, bfloat16 or float32, got {dtype}")
-    return DTYPE_IDS[dtype]
+    return found
 
 
 def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name: str) -> int:
@@ -39,11 +40,13 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
     one device, long enough -- and return its device's index.  (The library checks that codes
     are 16-byte aligned.)"""
     blocks = (n + BLOCK - 1) // BLOCK
-    if (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.is_cuda and scales.is_cuda
-            and codes.dtype in _CODE_DTYPES and scales.dtype in _SCALE_DTYPES and codes.is_contiguous()
-            and scales.is_contiguous() and codes.numel() >= rows * blocks * BLOCK_BYTES and scales.numel() >= rows * blocks):
+    if isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor):
         idx = codes.get_device()
-        if idx == scales.get_device():
+        if (idx >= 0 and scales.get_device() == idx
+                and (codes.dtype is torch.uint8 or codes.dtype in _CODE_DTYPES)
+                and (scales.dtype is torch.uint8 or scales.dtype in _SCALE_DTYPES)
+                and codes.is_contiguous() and scales.is_contiguous()
+                and codes.numel() >= rows * blocks * BLOCK_BYTES and scales.numel() >= rows * blocks):
             return idx
     for t, kind, dtypes, need in ((codes, "codes", _CODE_DTYPES, rows * blocks * BLOCK_BYTES),
                                   (scales, "scales", _SCALE_DTYPES, rows * blocks)):
@@ -60,13 +63,15 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
     raise ValueError(f"{name}_codes and {name}_scales must be on the same device")
 
 
-def call(fn, idx: int, args) -> None:
+def call(fn, idx: int, *args) -> None:
     """``fn(*args, stream)`` with device ``idx`` current, on its current stream."""
     if torch._C._cuda_getDevice() == idx:
-        _lib.check(fn(*args, _lib.current_stream_ptr(idx)))
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
-            _lib.check(fn(*args, _lib.current_stream_ptr(idx)))
+            status = fn(*args, _lib.current_stream_ptr(idx))
+    if status:
+        _lib.check(status)
 
 
 def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -87,7 +92,8 @@ def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         codes, scales = pack_mxfp4_tensor(x.cuda())
         return codes.cpu(), scales.cpu()
     lib = _lib.load()
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     *lead, n = x.shape
     blocks = (n + BLOCK - 1) // BLOCK
     device = x.device
@@ -95,7 +101,7 @@ def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scales = torch.empty(*lead, blocks, dtype=torch.uint8, device=device)
     total = x.numel()
     if total:
-        call(lib.feather_encode_mxfp4, device.index, (x.data_ptr(), src, codes.data_ptr(), scales.data_ptr(), total // n, n))
+        call(lib.feather_encode_mxfp4, device.index, x.data_ptr(), src, codes.data_ptr(), scales.data_ptr(), total // n, n)
     return codes, scales
 
 
@@ -108,16 +114,16 @@ def unpack_mxfp4_tensor(codes: torch.Tensor, scales: torch.Tensor, n: int | None
     dst = dtype_id(dtype, "dtype")
     if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
         raise TypeError("codes and scales must be torch.Tensors")
-    if codes.dim() == 0 or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != BLOCK_BYTES * scales.shape[-1]:
+    *lead, blocks = scales.shape or (-1,)
+    if codes.shape != (*lead, BLOCK_BYTES * blocks):
         raise ValueError(f"codes (..., 16 * blocks) and scales (..., blocks) do not match: "
                          f"{tuple(codes.shape)}, {tuple(scales.shape)}")
-    blocks = scales.shape[-1]
     n = blocks * BLOCK if n is None else int(n)
-    if blocks_of(n) != blocks or n < 0:
+    if n < 0 or (n + BLOCK - 1) // BLOCK != blocks:
         raise ValueError(f"n={n} does not have {blocks} blocks of {BLOCK}")
     rows = scales.numel() // blocks if blocks else 0
     idx = as_packed(codes, scales, rows, n, "m")
-    out = torch.empty(*codes.shape[:-1], n, dtype=dtype, device=codes.device)
+    out = torch.empty(*lead, n, dtype=dtype, device=codes.device)
     if rows:
-        call(_lib.load().feather_decode_mxfp4, idx, (codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows, n))
+        call(_lib.load().feather_decode_mxfp4, idx, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows, n)
     return out

@@ -22,7 +22,7 @@ MAX_VECTORS = 64
 def _shape(m_shape) -> tuple[int, int]:
     if len(m_shape) != 2:
         raise ValueError("m_shape must be the unpacked (M, N) of the matrix")
-    M, N = int(m_shape[0]), int(m_shape[1])
+    M, N = map(int, m_shape)
     if M < 0 or N < 0:
         raise ValueError("m_shape must not be negative")
     return M, N
@@ -52,8 +52,6 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
     shape = v.shape
     batch = 1 if dims == 1 else shape[0]
     if v_scales is None:
-        if not v.is_cuda:
-            raise ValueError("v must be a CUDA tensor: feather_b200 has no CPU path")
         v_dtype = dtype_id(v.dtype, "v (without v_scales)")
         if shape[-1] != N:
             raise ValueError(f"v has {shape[-1]} elements per vector, the matrix has N={N}")
@@ -66,7 +64,7 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
             raise ValueError(f"packed vectors of N={N} have {blocks_of(N) * BLOCK_BYTES} bytes each, got {shape[-1]}")
         v_dtype, scales_ptr = _lib.SRC_MXFP4, v_scales.data_ptr()
     if v.get_device() != idx:
-        raise ValueError("m and v must be on the same device")
+        raise ValueError("v must be a CUDA tensor on the matrix's device")
     if batch > MAX_VECTORS:
         raise ValueError(f"at most {MAX_VECTORS} vectors: pack them and use gemm_mxfp4_acc_fp32_gpu")
     if out is not None:
@@ -80,8 +78,8 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
         # one FP32 or two 16-bit vectors never need one
         need = 0 if batch == 1 or scales_ptr is not None else lib.feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype)
         ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
-        call(lib.feather_gemv_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr,
-                                           out.data_ptr(), ws.data_ptr() if need else None, M, N, batch))
+        call(lib.feather_gemv_mxfp4, idx, m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr,
+             out.data_ptr(), ws.data_ptr() if need else None, M, N, batch)
     return out
 
 
@@ -110,6 +108,6 @@ def gemm_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, x_cod
     else:
         out = torch.empty(*lead, M, dtype=out_dtype, device=x_codes.device)
     if M and batch:
-        call(_lib.load().feather_gemm_mxfp4, idx, (m_codes.data_ptr(), m_scales.data_ptr(), x_codes.data_ptr(),
-                                                   x_scales.data_ptr(), out.data_ptr(), dst, M, N, batch))
+        call(_lib.load().feather_gemm_mxfp4, idx, m_codes.data_ptr(), m_scales.data_ptr(), x_codes.data_ptr(),
+             x_scales.data_ptr(), out.data_ptr(), dst, M, N, batch)
     return out

@@ -86,17 +86,15 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     contiguous), or with ``mode`` "E5M2" / "E4M3" the FP8 words ``(heads, tokens, dim / 4)``: one
     head's ``result[h]`` is a packed (tokens, dim) matrix.  The angles are computed in 64 bits, so
     positions far into a context lose nothing."""
-    if not isinstance(x, torch.Tensor) or not isinstance(positions, torch.Tensor) or not isinstance(inv_freq, torch.Tensor):
+    if not (isinstance(x, torch.Tensor) and isinstance(positions, torch.Tensor) and isinstance(inv_freq, torch.Tensor)):
         raise TypeError("x, positions and inv_freq must be torch.Tensors")
     if layout not in LAYOUTS:
         raise NotImplementedError(f"layout {layout!r} not supported")
     out_mode = -1 if mode is None else _lib.mode_id(mode)
     dtype = dtype_id(x.dtype, "x")
-    if not (x.is_cuda and positions.is_cuda and inv_freq.is_cuda):
-        raise ValueError("x, positions and inv_freq must be CUDA tensors: feather_b200 has no CPU path")
     idx = x.get_device()
-    if positions.get_device() != idx or inv_freq.get_device() != idx:
-        raise ValueError("x, positions and inv_freq must be on the same device")
+    if idx < 0 or positions.get_device() != idx or inv_freq.get_device() != idx:
+        raise ValueError("x, positions and inv_freq must be CUDA tensors on one device: feather_b200 has no CPU path")
     if x.dim() != 3:
         raise ValueError("x must be (tokens, heads, dim)")
     tokens, heads, dim = x.shape
@@ -127,7 +125,7 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         if out.numel() != total // 4 or out.device != x.device:
             raise ValueError("out must hold heads * tokens * dim / 4 packed words on x's device")
     if total:
-        call(_lib.load().feather_rotary, idx,
-             (x.data_ptr(), dtype, token_stride, head_stride, positions.data_ptr(), 1 if wide else 0, inv_freq.data_ptr(),
-              out.data_ptr(), out_mode, tokens, heads, dim, rotated, LAYOUTS[layout], float(scale)))
+        call(_lib.load().feather_rotary, idx, x.data_ptr(), dtype, token_stride, head_stride, positions.data_ptr(),
+             1 if wide else 0, inv_freq.data_ptr(), out.data_ptr(), out_mode, tokens, heads, dim, rotated, LAYOUTS[layout],
+             scale)
     return out if mode is None or given else _tag(out, mode)

@@ -279,6 +279,24 @@ def test_rotary_packed(tokens, heads, dim, rotated, layout, dtype, mode, kind, h
     assert torch.equal(words.as_subclass(torch.Tensor).flatten().view(torch.int32), fb.pack_fp8_tensor(dense, mode).as_subclass(torch.Tensor).view(torch.int32))
 
 
+@pytest.mark.parametrize("mode", ["E5M2", "E4M3"])
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_rotary_packs_every_pattern_like_the_packer(dtype, mode):
+    # position 0 turns nothing and the second elements are zero, so the first ones are packed as they are: all 65536
+    # FP16 patterns, as FP16 and widened, and in FP32 the neighbours of each
+    x = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.float16)
+    if dtype == "fp32":
+        w = x.float().view(torch.int32)
+        x = torch.cat((w, w + 1, w - 1)).view(torch.float32)
+    heads = torch.zeros(1, x.numel() // 32, 64, dtype=x.dtype, device="cuda")
+    heads[0, :, :32] = x.view(-1, 32)
+    words = fb.rotary_gpu(heads, torch.zeros(1, dtype=torch.int64, device="cuda"), fb.rotary_frequencies(64), mode=mode)
+    got = words.as_subclass(torch.Tensor).view(torch.uint8).view(-1, 64)[:, :32].flatten()
+    want = fb.pack_fp8_tensor(x, mode).as_subclass(torch.Tensor).view(torch.uint8)
+    nan = x.isnan()                                    # the sign of a NaN is not kept by arithmetic
+    assert torch.equal(got[~nan], want[~nan]) and torch.equal(got[nan] & 127, want[nan] & 127)
+
+
 def test_rotary_strides_and_padding_rows_left_alone():
     gen = torch.Generator(device="cuda").manual_seed(1)
     qkv = torch.randn(9, 3, 4, 64, generator=gen, device="cuda", dtype=torch.float16)
