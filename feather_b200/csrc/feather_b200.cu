@@ -999,12 +999,18 @@ static int mx_gemm_launch(const unsigned char* x_codes, MxGemmArgs a, const Devi
     a.tiles_x = (a.batch + NT - 1) / NT;
     const long long tiles = (long long)a.tiles_m * a.tiles_x;
     if (tiles > 0x7FFFFFFFll - dev.sm_count) return FEATHER_ERR_TOO_LARGE;
-    // A stage takes about 0.23 us of an SM whose operands come from HBM, joining the partial sums
-    // about 1.8 us: split rows of at least 16 stages while the CTAs still run at once.  (Clusters
-    // of 8 do not: 16 of them took two waves, 10.6 against 6.6 us at 2048 x 5632 x 16.)
+    // A stage takes about 0.23 us of an SM whose operands come from HBM, joining the partial sums of
+    // four CTAs 1.2 us and 0.025 us for each column (2048 x 5632 x 16: 7.9 us whole, 6.8 in two, 5.6 in
+    // four; x 128: 10.0, 13.8, 10.6): four pay from 48 + NT < 6.8 stages on, two only for the few
+    // columns of dense vectors (8192 x 8192 x 4: 19.2 and 17.1 us).  Clusters of eight do not all run
+    // at once: 16 of them took two waves.
     const int stages = (a.blocks + kGmBlocks - 1) / kGmBlocks;
     a.split = 1;
-    while (a.split < 4 && stages >= 16 && tiles * a.split * 2 <= dev.sm_count) a.split *= 2;
+    if (DIGITS) {
+        while (a.split < 4 && stages >= 16 && tiles * a.split * 2 <= dev.sm_count) a.split *= 2;
+    } else if (tiles * 4 <= dev.sm_count && 48 + NT < 7 * stages) {
+        a.split = 4;
+    }
     CUtensorMap map_m, map_x, map_out = {};
     constexpr int kSize = OUT == kSrcF32 ? 4 : 2;
     a.bulk = !DIGITS && a.split == 1 && (long long)a.M * kSize % 16 == 0 && aligned(a.out, 16);
@@ -1063,7 +1069,7 @@ static int mx_gemm(const unsigned char* x_codes, const MxGemmArgs& a, const Devi
 }
 
 // Dense vectors as digits, eight at a time, through the product kernel.  `workspace` holds the
-// digits of one launch: 16 codes rows per vector, then their scales.
+// digits of one launch: their codes, then their scales.
 static long long mx_digits_bytes(int blocks, int vectors) { return (long long)vectors * kGmDigits * blocks * 17; }
 template <int VT>
 static int mx_gemv_digits(const MxGemvArgs& v, int batch, unsigned char* workspace, const DeviceInfo& dev, cudaStream_t s) {
@@ -1096,8 +1102,8 @@ static int mx_gemv_digits(const MxGemvArgs& v, int batch, unsigned char* workspa
             return FEATHER_ERR_LAUNCH;
         const int st = nv == 1   ? mx_gemm_launch<16, kSrcF32, true>(workspace, a, dev, s)
                        : nv == 2 ? mx_gemm_launch<32, kSrcF32, true>(workspace, a, dev, s)
-                       : nv <= 4 ? mx_gemm_launch<64, kSrcF32, true>(workspace, a, dev, s)
-                                 : mx_gemm_launch<128, kSrcF32, true>(workspace, a, dev, s);
+                       : nv <= 4 ? mx_gemm_launch<48, kSrcF32, true>(workspace, a, dev, s)
+                                 : mx_gemm_launch<96, kSrcF32, true>(workspace, a, dev, s);
         if (st != FEATHER_OK) return st;
     }
     return FEATHER_OK;

@@ -26,7 +26,7 @@
 // Dense vectors (DIGITS): a vector is first written as kGmDigits packed rows whose sum it is --
 // each row is the quantised remainder of the ones before it (mx_digits_kernel), at least two more
 // bits per row -- and its columns are added when they are stored.  With a matrix that is read
-// once anyway the extra columns cost nothing, and nothing of the matrix is decoded.
+// once anyway the extra columns cost little, and nothing of the matrix is decoded.
 #pragma once
 #include "attention_tc.cuh"   // descriptors, tensor-map copies, tensor-memory loads
 #include "mxfp4_codec.cuh"
@@ -133,19 +133,14 @@ __device__ __forceinline__ void gm_load_scales(uint32_t (&w)[8], const unsigned 
         const uint32_t shift = 8u * (uint32_t)(reinterpret_cast<uintptr_t>(row + k) & 3);
         const int left = blocks - k;             // bytes of this row still wanted, at least 1
         uint32_t x[9];
+        if (from >= begin && from + 36 <= all) { // no branch between the loads: they are in flight together
 #pragma unroll
-        for (int i = 0; i < 9; ++i) {
-            const unsigned char* p = from + 4 * i;
-            x[i] = 0u;
-            if (4 * i < left + 3) {
-                if (p >= begin && p + 4 <= all) {
-                    x[i] = __ldg(reinterpret_cast<const uint32_t*>(p));
-                } else {                         // a word across an end of the operand
+            for (int i = 0; i < 9; ++i) x[i] = __ldg(reinterpret_cast<const uint32_t*>(from) + i);
+        } else {                                 // at an end of the operand: byte by byte, and no further
+            for (int i = 0; i < 9; ++i) x[i] = 0u;
 #pragma unroll
-                    for (int b = 0; b < 4; ++b)
-                        if (p + b >= begin && p + b < all) x[i] |= (uint32_t)__ldg(p + b) << (8 * b);
-                }
-            }
+            for (int i = 0; i < 36; ++i)
+                if (from + i >= begin && from + i < all) x[i / 4] |= (uint32_t)__ldg(from + i) << (8 * (i % 4));
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -173,19 +168,22 @@ struct MxGemmArgs {
     long long N;
 };
 
-constexpr int kGmDigits = 16;
+constexpr int kGmDigits = 12;
 
-// Dense vectors to digits: row 16 n + d of (codes, scales) is the quantised remainder of vector n
-// after d rows.  Four threads per block, eight elements each; the remainder is exact in FP32 (an
-// element and its code's value are within a factor of two, or the code is zero).  After
-// kGmDigits rows it is at most 2^-32 of the block's largest element.  A block with an infinity
-// or a NaN gets scale 255 in row 0.
+// Dense vectors to digits: row kGmDigits n + d of (codes, scales) is the quantised remainder of vector
+// n after d rows.  Four threads per block, eight elements each; the remainder is exact in FP32 (an
+// element and its code's value are within a factor of two, or the code is zero).  A row leaves at
+// most a quarter of the block's largest remainder, so after all of them 2^-24 of its largest
+// element is left: one FP32 rounding of that.  (16 rows: 39.6 us for 8 vectors at 16384 x
+// 16384, 12 rows 38.8, before other steps.)  A block with an infinity or a NaN gets scale 255 in row 0.
 template <int VT>
 __global__ void __launch_bounds__(256)
 mx_digits_kernel(const void* __restrict__ v, uint32_t* __restrict__ codes, unsigned char* __restrict__ scales, long long N,
                  int blocks, int vectors) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // The product kernel behind this one may start once everything before this one is done: it reads
+    // the matrix before it waits for the digits.
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     typedef typename MxElem<VT>::type E;
     const int quads = blocks * vectors, i = blockIdx.x * blockDim.x + threadIdx.x;
     const bool mine = (i >> 2) < quads;
@@ -230,8 +228,8 @@ mx_digits_kernel(const void* __restrict__ v, uint32_t* __restrict__ codes, unsig
 
 // The digits' columns of a vector added up, the smallest digit first.
 __device__ __forceinline__ float gm_add_digits(uint32_t taddr) {
-    float r[kGmDigits];
-    tmem_ld<kGmDigits>(taddr, r);
+    float r[16];                                 // the last four are the next vector's
+    tmem_ld<16>(taddr, r);
     float x = r[kGmDigits - 1];
 #pragma unroll
     for (int d = kGmDigits - 2; d >= 0; --d) x += r[d];
@@ -243,14 +241,21 @@ __device__ __forceinline__ uint32_t gm_find_not_finite(const MxGemmArgs& g, int 
     uint32_t found = 0u;
     for (int c = 0; c < VECTORS && (x0 + c) * kGmDigits < g.batch; ++c) {
         const unsigned char* s = g.x_scales + (long long)(x0 + c) * kGmDigits * g.blocks;
-        bool bad = false;
-        for (int b = lane; b < g.blocks; b += 32) bad |= __ldg(s + b) == 255;
-        if (__any_sync(0xFFFFFFFFu, bad)) found |= 1u << c;
+        uint32_t top = 0u;
+        for (int b0 = lane; b0 - lane < g.blocks; b0 += 32 * 16) {     // sixteen loads in flight
+            uint32_t x[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) x[u] = b0 + 32 * u < g.blocks ? __ldg(s + b0 + 32 * u) : 0u;
+#pragma unroll
+            for (int u = 0; u < 16; ++u) top = max(top, x[u]);
+        }
+        if (__any_sync(0xFFFFFFFFu, top == 255u)) found |= 1u << c;
     }
     return found;
 }
-// Row m times such a vector: the blocks that hold what is not finite decide the result.
-__device__ __noinline__ float gm_not_finite(const MxGemmArgs& g, int m, int n) {
+// Row m times such a vector: the blocks that hold what is not finite decide the result.  (Not inlined,
+// it gives the kernel a stack frame, and that alone cost 7 of 36 us at 16384 x 16384 x 3.)
+__device__ __forceinline__ float gm_not_finite(const MxGemmArgs& g, int m, int n) {
     const unsigned char* s = g.x_scales + (long long)n * kGmDigits * g.blocks;
     float sum = 0.f;
     for (int b = 0; b < g.blocks; ++b) {
@@ -312,7 +317,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gm_smem + L::kBar + 8 * (2 * L::kStages + 8));
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // operands and result may be the previous kernel's
+    // Operands and result may be the previous kernel's -- but for the matrix of dense vectors: that
+    // kernel is mx_digits_kernel, which starts this one when all before it is done.
+    if (!DIGITS || warp != 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int n_tiles = g.tiles_m * g.tiles_x;
     const int all_steps = (g.blocks + kGmBlocks - 1) / kGmBlocks;
@@ -324,15 +331,25 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
-            int it = 0;
+            int it = 0, early = 0;               // stages so far; those whose rows of m are on their way already
+            if (DIGITS) {
+                early = tile0 < n_tiles ? min(L::kStages, n_step) : 0;
+                for (int k = 0; k < early; ++k) {
+                    mbar_arrive_expect_tx(full(k), (uint32_t)(L::kA + L::kB));
+                    tma_load_2d(sbase + k * (L::kA + L::kB), &map_m, (k_begin + k) * kGmBox, (tile0 / g.tiles_x) * kGmRows, full(k));
+                }
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+            }
             for (int tile = tile0; tile < n_tiles && ok; tile += tile_step) {
                 const int m0 = (tile / g.tiles_x) * kGmRows, x0 = (tile % g.tiles_x) * NT;
                 for (int k = 0; k < n_step && ok; ++k, ++it) {
                     const int s = it % L::kStages;
                     if (it >= L::kStages) ok = mbar_wait(empty(s), (uint32_t)((it / L::kStages - 1) & 1), g.status);
-                    mbar_arrive_expect_tx(full(s), (uint32_t)(L::kA + L::kB));
                     const uint32_t at = sbase + s * (L::kA + L::kB);
-                    tma_load_2d(at, &map_m, (k_begin + k) * kGmBox, m0, full(s));
+                    if (it >= early) {
+                        mbar_arrive_expect_tx(full(s), (uint32_t)(L::kA + L::kB));
+                        tma_load_2d(at, &map_m, (k_begin + k) * kGmBox, m0, full(s));
+                    }
                     tma_load_2d(at + L::kA, &map_x, (k_begin + k) * kGmBox, x0, full(s));
                 }
             }
@@ -375,14 +392,16 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
             }
         }
     } else if (warp < 6) {
-        // thread i: row i of m's tile, rows i (and i + 128) of x's.  The loads of the next group are
-        // issued behind the fence of this one: the fence would wait for them.
-        const int i = tid - 64;
+        // A thread takes row i of m's tile and rows i (and i + 128) of x's; the rows are dealt so that a
+        // warp's words are 128 consecutive bytes of a piece.  A group's loads are issued before the
+        // wait for the room of the one before it: the fence between that one's stores and the products
+        // waits for loads too, and then they have arrived.
+        const int i = (lane & 7) + 8 * (warp - 2) + 32 * (lane >> 3);
         const int at = (i & 31) * 16 + (i >> 5) * 4;
         const unsigned char* m_all = g.m_scales + (long long)g.M * g.blocks;
         const unsigned char* x_all = g.x_scales + (long long)g.batch * g.blocks;
-        uint32_t q[1 + L::kRowAtoms][8];
-        auto load = [&](int tile, int k) {
+        uint32_t q[2][1 + L::kRowAtoms][8];
+        auto load = [&](uint32_t (&q)[1 + L::kRowAtoms][8], int tile, int k) {
             const int m = (tile / g.tiles_x) * kGmRows + i, x = (tile % g.tiles_x) * NT + i;
             const bool there = tile < n_tiles;
 #pragma unroll
@@ -400,25 +419,33 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
             }
         };
         bool ok = true;
-        int grp = 0;
-        load(tile0, 0);
-        for (int tile = tile0; tile < n_tiles && ok; tile += tile_step) {
-            for (int k = 0; k < n_step && ok; k += kGmGroup, ++grp) {
-                if (grp >= 2) ok = mbar_wait(sf_empty(grp & 1), (uint32_t)((grp / 2 - 1) & 1), g.status);
-                unsigned char* sf = gm_smem + L::kSf + (grp & 1) * L::kSfGroup + at;
+        int grp = 0, l_tile = tile0, l_k = 0;
+        auto load_next = [&](uint32_t (&q)[1 + L::kRowAtoms][8]) {
+            load(q, l_tile, l_k);
+            if ((l_k += kGmGroup) >= n_step) l_k = 0, l_tile += tile_step;
+        };
+        load_next(q[0]);
+        const int n_grp = tile0 < n_tiles ? ((n_tiles - tile0 - 1) / tile_step + 1) * ((n_step + kGmGroup - 1) / kGmGroup) : 0;
+        for (int g0 = 0; g0 < n_grp && ok; g0 += 2) {
 #pragma unroll
-                for (int w = 0; w < 8; ++w) {    // word w: four blocks, half a stage
-                    unsigned char* to = sf + (w / 2) * L::kSfStage;
-                    *reinterpret_cast<uint32_t*>(to + 512 * (w & 1)) = q[0][w];
+            for (int u = 0; u < 2; ++u) {
+                if (grp < n_grp && ok) {
+                    load_next(q[u ^ 1]);
+                    if (grp >= 2) ok = mbar_wait(sf_empty(u), (uint32_t)((grp / 2 - 1) & 1), g.status);
+                    unsigned char* sf = gm_smem + L::kSf + u * L::kSfGroup + at;
 #pragma unroll
-                    for (int p = 0; p < L::kRowAtoms; ++p)
-                        *reinterpret_cast<uint32_t*>(to + 512 * (2 + L::kRowAtoms * (w & 1) + p)) = q[1 + p][w];
+                    for (int w = 0; w < 8; ++w) {    // word w: four blocks, half a stage
+                        unsigned char* to = sf + (w / 2) * L::kSfStage;
+                        *reinterpret_cast<uint32_t*>(to + 512 * (w & 1)) = q[u][0][w];
+#pragma unroll
+                        for (int p = 0; p < L::kRowAtoms; ++p)
+                            *reinterpret_cast<uint32_t*>(to + 512 * (2 + L::kRowAtoms * (w & 1) + p)) = q[u][1 + p][w];
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sf_full(u));
+                    ++grp;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sf_full(grp & 1));
-                if (k + kGmGroup < n_step) load(tile, k + kGmGroup);
-                else load(tile + tile_step, 0);
             }
         }
     }

@@ -132,6 +132,50 @@ def test_gemv(M, N, batch, vector):
     assert torch.equal(got, fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N), v_scales=v_scales))   # the same bits again
 
 
+def digits_bound(m, v):
+    """Several dense vectors on a large matrix go to the tensor cores as a sum of 12 packed rows: what is left of an
+    element is at most 2^-24 of its block's largest; N / 64 products in a row add into one FP32 sum per row and lose 2^-22 of the
+    products' size each; the rows' sums are at most 4/3 of the first, 11 additions and up to 3 of a cluster's parts round."""
+    blocks = -(-m.shape[1] // 32)
+    top = torch.nn.functional.pad(v.abs(), (0, blocks * 32 - v.shape[1])).view(v.shape[0], blocks, 32).amax(-1)
+    top = top.repeat_interleave(32, 1)[:, :v.shape[1]]
+    steps = math.ceil(m.shape[1] / 64) + 1
+    return top @ m.abs().T * 2.0 ** -24 + (v.abs() @ m.abs().T) * 2 * (steps * 2.0 ** -22 + 14 * 2.0 ** -24) + 1e-44
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("M,N,batch", [(9000, 4096, 3), (4100, 5000, 5), (2050, 5632, 8), (16400, 1024, 6), (3000, 3000, 11), (5000, 8192, 2)])
+def test_gemv_several_vectors_on_large_matrices(M, N, batch, dtype):
+    codes, scales = packed(M, N, M + N)
+    m = O.dequantise(codes, scales, N)
+    v = values(batch, N, M, DTYPES[dtype], spread=2.0)
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+    err, bound = (got.double() - v.double() @ m.T).abs(), digits_bound(m, v.double())
+    assert bool((err <= bound).all()), (err / bound).max()
+    assert torch.equal(got, fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N)))
+    # not finite: the vectors that hold it, with the signs that arithmetic gives; the others keep their bits
+    v = v.clone()
+    v[0, N - 1], v[1, 7], v[1, N // 2] = float("inf"), -float("inf"), float("nan")
+    if batch > 2:
+        v[2, 3], v[2, 4], v[2, N - 40] = float("inf"), float("inf"), -float("inf")
+    again = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+    want = v.double() @ m.T
+    assert torch.equal(again.isnan(), want.isnan()) and torch.equal(again[want.isinf()].double(), want[want.isinf()])
+    assert torch.equal(again[3:], got[3:])
+
+
+def test_digits_of_numbers_just_below_powers_of_two():
+    # the slowest expansion: every digit saturates and leaves a quarter
+    M, N = 9000, 4096
+    codes, scales = packed(M, N, 5, spread=0.0)
+    m = O.dequantise(codes, scales, N)
+    v = torch.full((3, N), 1 - 2.0 ** -24, device="cuda") * torch.exp2(torch.arange(N, device="cuda") // 32 % 5.0)
+    v[1] *= -1
+    v[2, ::2] = 2.0 ** -20
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+    assert bool(((got.double() - v.double() @ m.T).abs() <= digits_bound(m, v.double())).all())
+
+
 def test_gemv_large():
     M, N = 9000, 16384
     codes, scales = packed(M, N, 3)
