@@ -874,10 +874,15 @@ static int mx_encode_launch(const void* src, unsigned char* codes, unsigned char
         mx_encode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
             src, reinterpret_cast<uint32_t*>(codes), scales, words);
     } else {
-        const int blocks = mx_blocks(cols), runs = (blocks + kMxRun - 1) / kMxRun;
-        mx_encode_ragged_kernel<T><<<stream_grid(rows * runs, dev), 256, 0, s>>>(
-            reinterpret_cast<const typename MxElem<T>::type*>(src), reinterpret_cast<uint32_t*>(codes), scales, rows,
-            cols, blocks, runs);
+        typedef typename MxElem<T>::type E;
+        const uint32_t words_row = 4u * (uint32_t)mx_blocks(cols);
+        const long long words = rows * words_row;
+        const unsigned grid = stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev);
+        uint32_t* to = reinterpret_cast<uint32_t*>(codes);
+        if (sizeof(E) == 2 && cols % 2 == 0 && aligned(src, 4))
+            mx_encode_rows_kernel<T, 4><<<grid, 256, 0, s>>>(static_cast<const E*>(src), to, scales, words, cols, words_row);
+        else
+            mx_encode_rows_kernel<T, sizeof(E)><<<grid, 256, 0, s>>>(static_cast<const E*>(src), to, scales, words, cols, words_row);
     }
     return launch_status();
 }
@@ -890,9 +895,15 @@ static int mx_decode_launch(const unsigned char* codes, const unsigned char* sca
         mx_decode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
             reinterpret_cast<const uint32_t*>(codes), scales, dst, words);
     } else {
-        const int blocks = mx_blocks(cols), runs = (blocks + kMxRun - 1) / kMxRun;
-        mx_decode_ragged_kernel<T><<<stream_grid(rows * runs, dev), 256, 0, s>>>(
-            codes, scales, reinterpret_cast<typename MxElem<T>::type*>(dst), rows, cols, blocks, runs);
+        typedef typename MxElem<T>::type E;
+        const int blocks = mx_blocks(cols), runs = (blocks + 2 * kMxRun - 1) / (2 * kMxRun);
+        const unsigned grid = stream_grid(rows * runs, dev);
+        bool paired = false;
+        if constexpr (sizeof(E) == 2) {
+            paired = cols % 2 == 0 && aligned(dst, 4);
+            if (paired) mx_decode_rows_kernel<T, true><<<grid, 256, 0, s>>>(codes, scales, static_cast<E*>(dst), rows, cols, blocks, runs);
+        }
+        if (!paired) mx_decode_rows_kernel<T, false><<<grid, 256, 0, s>>>(codes, scales, static_cast<E*>(dst), rows, cols, blocks, runs);
     }
     return launch_status();
 }

@@ -154,37 +154,59 @@ mx_encode_kernel(const void* __restrict__ src, uint32_t* __restrict__ codes, uns
     }
 }
 
-// Any row length and alignment: a warp takes kMxRun consecutive blocks of a row, one element of
-// each per lane (consecutive loads whatever the row's start), the maximum with one warp reduction.
-constexpr int kMxRun = 8;
-template <int T>
+// Any row length and alignment: the same four threads to a block, each finding its row by a division
+// and loading its eight elements W bytes at a time (what the rows' alignment allows); the
+// loads of a warp touch the same lines one after the other and hit in L1.
+template <int T, int W>
 __global__ void __launch_bounds__(256)
-mx_encode_ragged_kernel(const typename MxElem<T>::type* __restrict__ src, uint32_t* __restrict__ codes,
-                        unsigned char* __restrict__ scales, long long rows, long long cols, int blocks_row, int runs_row) {
+mx_encode_rows_kernel(const typename MxElem<T>::type* __restrict__ src, uint32_t* __restrict__ codes,
+                      unsigned char* __restrict__ scales, long long n_words, long long cols, uint32_t words_row) {
     const int lane = threadIdx.x & 31;
-    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, runs = rows * runs_row;
-    for (long long run = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; run < runs; run += warps) {
-        const long long row = runs >> 32 ? run / runs_row : (uint32_t)run / (uint32_t)runs_row;
-        const int b0 = (int)(run - row * runs_row) * kMxRun;
-        const typename MxElem<T>::type* from = src + row * cols;
-        float x[kMxRun];
+    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
+    const long long warp = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    constexpr int kPer = W / (int)sizeof(typename MxElem<T>::type);   // elements of a load
+    for (long long base = warp * (32 * kMxSteps); base < n_words; base += warps * (32 * kMxSteps)) {
+        float x[kMxSteps][8];
 #pragma unroll
-        for (int u = 0; u < kMxRun; ++u) {
-            const long long col = (long long)(b0 + u) * kMxBlock + lane;
-            x[u] = col < cols ? MxElem<T>::get(from[col]) : 0.f;
+        for (int u = 0; u < kMxSteps; ++u) {
+            const long long w = min(base + 32 * u + lane, n_words - 1);
+            const long long row = n_words >> 32 ? w / words_row : (uint32_t)w / words_row;
+            const long long col = (w - row * words_row) * 8;
+            const typename MxElem<T>::type* p = src + row * cols + col;
+            if (col + 8 <= cols) {
+#pragma unroll
+                for (int k = 0; k < 8; k += kPer) {
+                    if constexpr (kPer == 1) {
+                        x[u][k] = MxElem<T>::get(p[k]);
+                    } else {
+                        const uint32_t pair = *reinterpret_cast<const uint32_t*>(p + k);
+                        x[u][k] = MxElem<T>::get((unsigned short)(pair & 0xFFFFu));
+                        x[u][k + 1] = MxElem<T>::get((unsigned short)(pair >> 16));
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[u][k] = col + k < cols ? MxElem<T>::get(p[k]) : 0.f;
+            }
         }
 #pragma unroll
-        for (int u = 0; u < kMxRun; ++u) {
-            if (b0 + u >= blocks_row) break;
-            const uint32_t b = mx_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(x[u]) & 0x7FFFFFFFu));
-            const float y[8] = {x[u] * mx_to_grid(b), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            uint32_t c = (b == 255u ? 0u : mx_encode8(y) & 0xFu) << (4 * (lane & 7));
-            c |= __shfl_xor_sync(0xFFFFFFFFu, c, 1);
-            c |= __shfl_xor_sync(0xFFFFFFFFu, c, 2);
-            c |= __shfl_xor_sync(0xFFFFFFFFu, c, 4);
-            const long long blk = row * blocks_row + b0 + u;
-            if ((lane & 7) == 0) codes[blk * 4 + (lane >> 3)] = c;
-            if (lane == 0) scales[blk] = (unsigned char)b;
+        for (int u = 0; u < kMxSteps; ++u) {
+            const long long w = base + 32 * u + lane;
+            uint32_t m = 0u;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(x[u][k]) & 0x7FFFFFFFu);
+            m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+            m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+            const uint32_t b = mx_scale_byte(m);
+            const float f = mx_to_grid(b);
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = x[u][k] * f;
+            const uint32_t c = mx_encode8(y);
+            if (w < n_words) {
+                codes[w] = b == 255u ? 0u : c;
+                if ((lane & 3) == 0) scales[w >> 2] = (unsigned char)b;
+            }
         }
     }
 }
@@ -247,32 +269,41 @@ mx_decode_kernel(const uint32_t* __restrict__ codes, const unsigned char* __rest
     }
 }
 
-// Any row length and alignment: a warp takes kMxRun consecutive blocks of a row, consecutive lanes
-// consecutive elements.
-template <int T>
+// Any row length and alignment: a warp takes kMxRun consecutive pairs of blocks of a row, a lane two
+// consecutive elements (a byte) of each, so that its stores are consecutive; PAIRED: rows of
+// an even number of 16-bit elements, stored two at a time.
+constexpr int kMxRun = 4;            // as many as mx_decode8 takes
+template <int T, bool PAIRED>
 __global__ void __launch_bounds__(256)
-mx_decode_ragged_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                        typename MxElem<T>::type* __restrict__ dst, long long rows, long long cols, int blocks_row,
-                        int runs_row) {
+mx_decode_rows_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                      typename MxElem<T>::type* __restrict__ dst, long long rows, long long cols, int blocks_row,
+                      int runs_row) {
     const int lane = threadIdx.x & 31;
     const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, runs = rows * runs_row;
     for (long long run = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; run < runs; run += warps) {
         const long long row = runs >> 32 ? run / runs_row : (uint32_t)run / (uint32_t)runs_row;
-        const int b0 = (int)(run - row * runs_row) * kMxRun;
+        const int b0 = (int)(run - row * runs_row) * (2 * kMxRun) + (lane >> 4);
         const long long blk = row * blocks_row + b0;
-        uint32_t pair[kMxRun], s[kMxRun];
+        uint32_t pairs = 0u, h[4], s[kMxRun];
 #pragma unroll
         for (int u = 0; u < kMxRun; ++u) {
-            const bool there = b0 + u < blocks_row;
-            pair[u] = there ? codes[(blk + u) * 16 + (lane >> 1)] : 0u;
-            s[u] = there ? scales[blk + u] : 0u;
+            const bool there = b0 + 2 * u < blocks_row;
+            pairs |= (there ? (uint32_t)codes[(blk + 2 * u) * 16 + (lane & 15)] : 0u) << (8 * u);
+            s[u] = there ? scales[blk + 2 * u] : 0u;
         }
+        mx_decode8(pairs, h);
 #pragma unroll
         for (int u = 0; u < kMxRun; ++u) {
-            const long long col = (long long)(b0 + u) * kMxBlock + lane;
-            uint32_t h[4];
-            mx_decode8(lane & 1 ? pair[u] >> 4 : pair[u], h);
-            if (col < cols) dst[row * cols + col] = MxElem<T>::put(h2_to_f2(h[0]).x * mx_scale_value(s[u]));
+            const long long col = (long long)(b0 + 2 * u) * kMxBlock + 2 * (lane & 15);
+            const float2 x = h2_to_f2(h[u]);
+            const float f = mx_scale_value(s[u]);
+            typename MxElem<T>::type* to = dst + row * cols + col;
+            if constexpr (PAIRED) {
+                if (col < cols) *reinterpret_cast<uint32_t*>(to) = mx_put2<T>(x.x * f, x.y * f);
+            } else {
+                if (col < cols) to[0] = MxElem<T>::put(x.x * f);
+                if (col + 1 < cols) to[1] = MxElem<T>::put(x.y * f);
+            }
         }
     }
 }
