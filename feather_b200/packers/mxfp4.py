@@ -37,7 +37,7 @@ def dtype_id(dtype: torch.dtype, name: str) -> int:
 
 def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name: str) -> int:
     """Validate a packed operand of ``rows`` rows of ``n`` elements -- CUDA, contiguous, bytes,
-    one device, long enough -- and return its device's index.  (The library checks that codes
+    one device, long enough, rows of the right length -- and return its device's index.  (The library checks that codes
     are 16-byte aligned.)"""
     blocks = (n + BLOCK - 1) // BLOCK
     if isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor):
@@ -46,7 +46,8 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
                 and (codes.dtype is torch.uint8 or codes.dtype in _CODE_DTYPES)
                 and (scales.dtype is torch.uint8 or scales.dtype in _SCALE_DTYPES)
                 and codes.is_contiguous() and scales.is_contiguous()
-                and codes.numel() >= rows * blocks * BLOCK_BYTES and scales.numel() >= rows * blocks):
+                and codes.numel() >= rows * blocks * BLOCK_BYTES and scales.numel() >= rows * blocks
+                and (blocks == 0 or not (codes.shape[-1] % (blocks * BLOCK_BYTES) or scales.shape[-1] % blocks))):
             return idx
     for t, kind, dtypes, need in ((codes, "codes", _CODE_DTYPES, rows * blocks * BLOCK_BYTES),
                                   (scales, "scales", _SCALE_DTYPES, rows * blocks)):
@@ -60,6 +61,8 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
             raise ValueError(f"{name}_{kind} must be contiguous")
         if t.numel() < need:
             raise ValueError(f"{name}_{kind} holds {t.numel()} bytes, {rows}x{n} needs {need}")
+        if blocks and t.shape[-1] % (need // rows if rows else 1):
+            raise ValueError(f"{name}_{kind} of shape {tuple(t.shape)} does not have rows of {need // rows} bytes (n={n})")
     raise ValueError(f"{name}_codes and {name}_scales must be on the same device")
 
 

@@ -111,7 +111,8 @@ def gemv_bound(m, v, split):
 
 @pytest.mark.parametrize("vector", ["fp16", "bf16", "fp32", "mxfp4"])
 @pytest.mark.parametrize("M,N,batch", [(1, 1, 1), (1, 32, 1), (17, 33, 1), (16, 128, 2), (3, 4000, 1), (256, 2048, 1), (250, 2080, 3),
-                                       (2400, 256, 1), (2500, 100, 5), (4800, 4096, 1), (40, 30000, 2), (100, 1024, 8), (33, 640, 11)])
+                                       (2400, 256, 1), (2500, 100, 5), (4800, 4096, 1), (40, 30000, 2), (100, 1024, 8), (33, 640, 11),
+                                       (100, 8192, 8), (21400, 20000, 2)])
 def test_gemv(M, N, batch, vector):
     codes, scales = packed(M, N, M + N)
     m = O.dequantise(codes, scales, N)
@@ -186,16 +187,55 @@ def test_gemv_large():
         assert bool(((got.double() - v.double() @ m.T).abs() <= gemv_bound(m, v.double(), dtype == "fp32")).all())
 
 
-def test_gemv_more_rows_than_partial_sums_fit():
+@pytest.mark.parametrize("M,batch", [(148 * 16 * 260 + 5, 1), (230001, 8)])
+def test_gemv_more_rows_than_partial_sums_fit(M, batch):
     # one column tile, so that every warp takes rows; more 16-row groups per CTA than one round of partial sums
-    M, N = 148 * 16 * 2 * 400 + 5, 32
+    N = 32
     gen = torch.Generator(device="cuda").manual_seed(8)
     codes = torch.randint(0, 256, (M, 16), generator=gen, device="cuda").to(torch.uint8)
     scales = torch.randint(120, 130, (M, 1), generator=gen, device="cuda").to(torch.uint8)
-    v = values(1, N, 4, torch.bfloat16)
+    v = values(batch, N, 4, torch.bfloat16)
     m = O.dequantise(codes, scales, N)
     got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
     assert bool(((got.double() - v.double() @ m.T).abs() <= gemv_bound(m, v.double(), False)).all())
+
+
+@pytest.mark.parametrize("N", [2048, 5000, 2050])
+def test_products_of_operands_off_the_grid(N):
+    # scales that start on odd bytes and end where their buffer ends, vectors that start off the 16-byte grid
+    M, batch = 300, 70
+    codes, scales = packed(M, N, 1, spread=1.0)
+    x, x_scales = packed(batch, N, 2, spread=1.0)
+
+    def odd(t):
+        buf = torch.full((t.numel() + 3,), 255, dtype=torch.uint8, device="cuda")     # NaN scales on either side
+        out = buf[3:].view(t.shape)
+        out.copy_(t)
+        return out
+    want = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N))
+    assert bool(want.isfinite().all())
+    assert torch.equal(fb.gemm_mxfp4_acc_fp32_gpu(codes, odd(scales), x, odd(x_scales), (M, N)), want)
+    v = values(1, N, 3, torch.float16)
+    w = torch.empty(N + 1, dtype=torch.float16, device="cuda")[1:].copy_(v[0])
+    assert w.data_ptr() % 16
+    assert torch.equal(fb.gemv_mxfp4_acc_fp32_gpu(codes, odd(scales), w, (M, N)), fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v[0], (M, N)))
+    assert torch.equal(fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, x[0], (M, N), v_scales=odd(x_scales)[0]),
+                       fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, x[0], (M, N), v_scales=x_scales[0]))
+    out = torch.full((batch * M + 1,), 7.0, device="cuda", dtype=torch.bfloat16)      # a result off the grid, and what is behind it
+    got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N), out_dtype=torch.bfloat16, out=out[1:])
+    assert torch.equal(got.view(batch, M), want.to(torch.bfloat16)) and out[0] == 7.0
+
+
+def test_products_leave_what_is_behind_their_result():
+    for M, batch in ((130, 33), (128, 40), (500, 129), (40, 1)):
+        codes, scales = packed(M, 320, 1)
+        x, x_scales = packed(batch, 320, 2)
+        out = torch.full((batch + 3, M), 7.0, device="cuda")
+        fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, 320), out=out[:batch])
+        assert bool((out[batch:] == 7.0).all()) and bool((out[:batch] != 7.0).any())
+        out.fill_(7.0)
+        fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, torch.randn(320, device="cuda"), (M, 320), out=out[0])
+        assert bool((out[1:] == 7.0).all())
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -262,6 +302,24 @@ def test_gemm_every_place_and_scale_is_its_own():
     got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N))
     e = scales[torch.arange(M, device="cuda"), k // 32].int()[None, :] + x_scales.int()[:, k // 32]
     assert torch.equal(got, torch.exp2((e - 254).float()))
+
+
+def test_gemm_scales_of_the_whole_range():
+    # one element per row, scales from 2^-127 to 2^127: sums inside FP32's normal range are exact, larger ones infinite,
+    # smaller ones at most the smallest normal number off
+    M, N, batch = 256, 256, 160
+    codes = torch.zeros(M, N // 2, dtype=torch.uint8, device="cuda")
+    k = (torch.arange(M, device="cuda") * 37) % N
+    codes[torch.arange(M, device="cuda"), k // 2] = torch.where(k % 2 == 0, 2, 32).to(torch.uint8)
+    x = torch.full((batch, N // 2), 0x22, dtype=torch.uint8, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    scales = torch.randint(0, 255, (M, N // 32), generator=gen, device="cuda").to(torch.uint8)
+    x_scales = torch.randint(0, 255, (batch, N // 32), generator=gen, device="cuda").to(torch.uint8)
+    got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N))
+    want = O.dequantise(x, x_scales, N) @ O.dequantise(codes, scales, N).T
+    normal = (want >= 2.0 ** -126) & (want < 2.0 ** 128)
+    assert torch.equal(got[normal].double(), want[normal]) and bool(got[want >= 2.0 ** 128].isinf().all())
+    assert bool((got[want < 2.0 ** -126].double() <= 2.0 ** -126).all())
 
 
 def test_gemm_nan_scales_stay_in_their_row():
@@ -420,6 +478,42 @@ def test_captured_and_replayed_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(got, chain()))
 
 
+def test_two_streams_at_once():
+    M, N = 3000, 4096
+    w = packed(M, N, 1)
+    jobs = []
+    for i in range(2):
+        x = torch.randn(6, N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i))
+        want = [fb.gemv_mxfp4_acc_fp32_gpu(*w, x, (M, N)), fb.gemm_mxfp4_acc_fp32_gpu(*w, *fb.pack_mxfp4_tensor(x), (M, N))]
+        jobs.append((torch.cuda.Stream(), x, want))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (stream, x, _) in enumerate(jobs):
+            with torch.cuda.stream(stream):
+                got[i] += [fb.gemv_mxfp4_acc_fp32_gpu(*w, x, (M, N)), fb.gemm_mxfp4_acc_fp32_gpu(*w, *fb.pack_mxfp4_tensor(x), (M, N))]
+    torch.cuda.synchronize()
+    for (_, _, want), ys in zip(jobs, got):
+        assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(ys))
+
+
+def test_packed_right_before_it_is_multiplied():
+    # operands written by the call just before, several times over in the same buffers of the allocator
+    M, N = 5000, 4096
+    x = torch.randn(4, N, device="cuda")
+    for seed in range(4):
+        a = torch.randn(M, N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+        torch.cuda.synchronize()
+        codes, scales = fb.pack_mxfp4_tensor(a)
+        y = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, x, (M, N))
+        z = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, *fb.pack_mxfp4_tensor(x), (M, N))
+        one = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, x[0], (M, N))
+        torch.cuda.synchronize()
+        assert torch.equal(y, fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, x, (M, N)))
+        assert torch.equal(z, fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, *fb.pack_mxfp4_tensor(x), (M, N)))
+        assert torch.equal(one, fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, x[0], (M, N)))
+
+
 def test_refusals_on_the_gpu():
     codes, scales = packed(8, 64, 1)
     x = torch.randn(64, device="cuda")
@@ -428,7 +522,8 @@ def test_refusals_on_the_gpu():
     for bad in (dict(v=x[:63]), dict(v=torch.randn(1, 2, 64, device="cuda")), dict(v=torch.randn(128, device="cuda")[::2]),
                 dict(m_shape=(9, 64)), dict(m_shape=(8, 65)), dict(m_scales=scales[:4]), dict(m_codes=codes[:, ::2]),
                 dict(out=torch.empty(9, device="cuda")), dict(out=torch.empty(8, device="cuda", dtype=torch.float16)),
-                dict(v=torch.randn(65, 64, device="cuda")), dict(v_scales=scales[0]),
+                dict(v=torch.randn(65, 64, device="cuda")), dict(v_scales=scales[0]), dict(v=x.cpu()),
+                dict(m_scales=torch.zeros(8, 3, dtype=torch.uint8, device="cuda")), dict(m_codes=torch.zeros(8, 33, dtype=torch.uint8, device="cuda")),
                 dict(m_codes=torch.zeros(8 * 32 + 8, dtype=torch.uint8, device="cuda")[8:].view(8, 32))):
         with pytest.raises(ValueError):
             fb.gemv_mxfp4_acc_fp32_gpu(**{**ok, **bad})
