@@ -1120,14 +1120,21 @@ static int mx_gemv_digits(const MxGemvArgs& v, int batch, unsigned char* workspa
     return FEATHER_OK;
 }
 
+// Elements of a vector access that these sizes, strides and addresses allow: `most` or half of it, else 1.
+static int rotary_width(const RotaryArgs& a, int mode, int size, int most) {
+    for (int v = most; v >= 4; v /= 2)
+        if (aligned(a.x, (uintptr_t)v * size) && aligned(a.out, mode < 0 ? (uintptr_t)v * size : (uintptr_t)v) &&
+            (a.rotated / 2) % v == 0 && a.dim % v == 0 && a.token_stride % v == 0 && a.head_stride % v == 0)
+            return v;
+    return 1;
+}
+
 template <int T, int MODE>
 static int rotary_launch(RotaryArgs a, const DeviceInfo& dev, cudaStream_t s) {
     constexpr int kWide = T == kSrcF32 ? 4 : 8;
-    const bool wide = aligned(a.x, 16) && aligned(a.out, MODE < 0 ? 16 : kWide) && (a.rotated / 2) % kWide == 0 &&
-                      a.dim % kWide == 0 && a.token_stride % kWide == 0 && a.head_stride % kWide == 0;
-    const int v = wide ? kWide : 1;
+    const int v = rotary_width(a, MODE, T == kSrcF32 ? 4 : 2, kWide);
     const long long items = (long long)a.heads * (a.rotated / 2 / v + (a.dim - a.rotated + 2 * v - 1) / (2 * v));
-    // tiles of up to eight tokens while there are six CTAs per SM; few tokens share their heads out
+    // tiles of up to kRotTile tokens while there are six CTAs per SM; few tokens share their heads out
     const long long full = 6ll * dev.sm_count, rounds = (items + kRotThreads - 1) / kRotThreads;
     long long tile = a.tokens / full;
     tile = tile < 1 ? 1 : tile < kRotTile ? tile : kRotTile;
@@ -1140,7 +1147,8 @@ static int rotary_launch(RotaryArgs a, const DeviceInfo& dev, cudaStream_t s) {
     gy = (items + per - 1) / per;
     a.items_each = (int)per;
     const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (wide) rotary_kernel<T, MODE, kWide><<<grid, kRotThreads, 0, s>>>(a);
+    if (v == kWide) rotary_kernel<T, MODE, kWide><<<grid, kRotThreads, 0, s>>>(a);
+    else if (v == 4) rotary_kernel<T, MODE, 4><<<grid, kRotThreads, 0, s>>>(a);
     else rotary_kernel<T, MODE, 1><<<grid, kRotThreads, 0, s>>>(a);
     return launch_status();
 }

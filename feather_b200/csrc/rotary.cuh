@@ -36,15 +36,19 @@ __device__ __forceinline__ float2 rotary_turn(double position, double inv_freq) 
 // V consecutive elements as loaded, and widened: what waits for its turn takes few registers.
 template <int T, int V>
 struct RotaryRaw {
-    static constexpr int kWords = V == 1 ? 1 : 4;
-    uint32_t w[kWords];
+    static constexpr int kBytes = V * (int)sizeof(typename MxElem<T>::type);   // 16, 8, or one element's
+    uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
     __device__ __forceinline__ void load(const typename MxElem<T>::type* p) {
-        if constexpr (V == 1) {
-            if constexpr (T == kSrcF32) w[0] = __float_as_uint(*p);
-            else w[0] = *p;
-        } else {
+        if constexpr (kBytes == 16) {
             const uint4 a = *reinterpret_cast<const uint4*>(p);
             w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        } else if constexpr (kBytes == 8) {
+            const uint2 a = *reinterpret_cast<const uint2*>(p);
+            w[0] = a.x; w[1] = a.y;
+        } else if constexpr (T == kSrcF32) {
+            w[0] = __float_as_uint(*p);
+        } else {
+            w[0] = *p;
         }
     }
     __device__ __forceinline__ void widen(float (&x)[V]) const {
@@ -98,14 +102,11 @@ __device__ __forceinline__ void rotary_store(void* out, long long at, const floa
         }
     } else {
         typename MxElem<T>::type* p = reinterpret_cast<typename MxElem<T>::type*>(out) + at;
-        if constexpr (V == 1) {
-            *p = MxElem<T>::put(y[0]);
-        } else if constexpr (T == kSrcF32) {
-            *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
-        } else {
-            *reinterpret_cast<uint4*>(p) = make_uint4(mx_put2<T>(y[0], y[1]), mx_put2<T>(y[2], y[3]),
-                                                      mx_put2<T>(y[4], y[5]), mx_put2<T>(y[6], y[7]));
-        }
+        if constexpr (V == 1) *p = MxElem<T>::put(y[0]);
+        else if constexpr (T == kSrcF32) *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+        else if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(mx_put2<T>(y[0], y[1]), mx_put2<T>(y[2], y[3]));
+        else *reinterpret_cast<uint4*>(p) = make_uint4(mx_put2<T>(y[0], y[1]), mx_put2<T>(y[2], y[3]),
+                                                       mx_put2<T>(y[4], y[5]), mx_put2<T>(y[6], y[7]));
     }
 }
 
@@ -123,7 +124,8 @@ struct RotaryArgs {
 // A CTA takes `tile` consecutive tokens (blockIdx.x) and a share of their heads (blockIdx.y): first the
 // tile's angles, then, without another barrier, items of two V-element vectors -- a pair of vectors
 // that turn into each other, or 2 V elements that pass through -- kRotBatch tokens of an item in
-// flight per thread.  V = 16 bytes of the input type where sizes, strides and addresses allow, else 1.
+// flight per thread.  V = 16 bytes of the input type
+// where sizes, strides and addresses allow, else (16-bit types) 8 bytes, else 1.
 template <int T, int MODE, int V>
 __global__ void __launch_bounds__(kRotThreads, 4)
 rotary_kernel(const RotaryArgs a) {

@@ -348,7 +348,8 @@ def rotary_bound(x, positions, inv_freq, layout, scale, dtype):
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("tokens,heads,dim,rotated,start", [(1, 1, 2, 2, 0), (1, 36, 64, 64, 100003), (5, 3, 80, 40, 7), (3, 2, 96, 34, 2 ** 20),
-                                                            (130, 4, 128, 64, 2 ** 31 - 131), (17, 1, 1024, 1024, 50), (2, 5, 33, 6, 9)])
+                                                            (130, 4, 128, 64, 2 ** 31 - 131), (17, 1, 1024, 1024, 50), (2, 5, 33, 6, 9),
+                                                            (1300, 7, 80, 40, 3), (40, 2, 88, 24, 3)])
 def test_rotary(tokens, heads, dim, rotated, start, dtype, layout):
     gen = torch.Generator(device="cuda").manual_seed(tokens + dim)
     x = torch.randn(tokens, heads, dim, generator=gen, device="cuda").to(DTYPES[dtype])
@@ -365,7 +366,8 @@ def test_rotary(tokens, heads, dim, rotated, start, dtype, layout):
 
 @pytest.mark.parametrize("mode,kind,half_step,tiny", [("E5M2", torch.float8_e5m2, 2.0 ** -3, 2.0 ** -17), ("E4M3", torch.float8_e4m3fn, 2.0 ** -4, 2.0 ** -10)])
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("tokens,heads,dim,rotated,layout", [(1, 4, 64, 64, "half"), (33, 3, 128, 64, "interleaved"), (7, 2, 20, 6, "half")])
+@pytest.mark.parametrize("tokens,heads,dim,rotated,layout", [(1, 4, 64, 64, "half"), (33, 3, 128, 64, "interleaved"), (7, 2, 20, 6, "half"),
+                                                              (50, 3, 80, 40, "interleaved"), (9, 1, 88, 24, "half")])
 def test_rotary_packed(tokens, heads, dim, rotated, layout, dtype, mode, kind, half_step, tiny):
     gen = torch.Generator(device="cuda").manual_seed(dim)
     x = torch.randn(tokens, heads, dim, generator=gen, device="cuda").to(DTYPES[dtype])
