@@ -1134,11 +1134,17 @@ static int rotary_launch(RotaryArgs a, const DeviceInfo& dev, cudaStream_t s) {
     constexpr int kWide = T == kSrcF32 ? 4 : 8;
     const int v = rotary_width(a, MODE, T == kSrcF32 ? 4 : 2, kWide);
     const long long items = (long long)a.heads * (a.rotated / 2 / v + (a.dim - a.rotated + 2 * v - 1) / (2 * v));
-    // tiles of up to kRotTile tokens while there are six CTAs per SM; few tokens share their heads out
-    const long long full = 6ll * dev.sm_count, rounds = (items + kRotThreads - 1) / kRotThreads;
-    long long tile = a.tokens / full;
-    tile = tile < 1 ? 1 : tile < kRotTile ? tile : kRotTile;
-    while (tile > 1 && tile * (a.rotated / 2) > kRotAngles) tile /= 2;
+    // The tile whose waves of four CTAs per SM are the shortest, a tile's angles counting as 0.7 of a
+    // token; few tokens share their heads out.  (Against tiles of 4 throughout: 12583 tokens of
+    // 25 x 80 21.0 -> 18.9 us, 8192 of 32 x 128 the same.)
+    const long long full = 4ll * dev.sm_count, rounds = (items + kRotThreads - 1) / kRotThreads;
+    long long tile = 1;
+    double best = 0.0;
+    for (int t = 1; t <= kRotTile && t * (a.rotated / 2) <= kRotAngles; ++t) {
+        const long long ctas = (a.tokens + t - 1) / t;
+        const double cost = (double)((ctas + full - 1) / full) * (t + 0.7);
+        if (t == 1 || cost < best) best = cost, tile = t;
+    }
     a.tile = (int)tile;
     const long long gx = (a.tokens + tile - 1) / tile;
     if (gx > 0x7FFFFFFFll) return FEATHER_ERR_TOO_LARGE;
