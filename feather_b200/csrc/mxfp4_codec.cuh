@@ -111,7 +111,8 @@ __device__ __forceinline__ uint32_t mx_load8(const void* src, long long e, float
 // Rows of whole blocks, 16-byte aligned: the matrix is a flat run of blocks.  Four threads
 // take a block, eight elements each (16- or 2 x 16-byte loads), and agree on the block's
 // maximum with two shuffles; a warp takes kMxSteps runs of 256 elements per trip.  Bound by
-// HBM: it reads every element once and writes 17/32 byte for each.
+// HBM: it reads every element once and writes 17/32 byte for each; 16384 x 8192 FP16 57.2 us
+// (5.9 TB/s).
 constexpr int kMxSteps = 4;
 template <int T>
 __global__ void __launch_bounds__(256)
@@ -156,7 +157,8 @@ mx_encode_kernel(const void* __restrict__ src, uint32_t* __restrict__ codes, uns
 
 // Any row length and alignment: the same four threads to a block, each finding its row by a division
 // and loading its eight elements W bytes at a time (what the rows' alignment allows); the
-// loads of a warp touch the same lines one after the other and hit in L1.
+// loads of a warp touch the same lines one after the other and hit in L1.  5001 x 2050 FP16 10.8
+// us; a warp per block with one element per lane took 26.7 (three quarters of it instructions).
 template <int T, int W>
 __global__ void __launch_bounds__(256)
 mx_encode_rows_kernel(const typename MxElem<T>::type* __restrict__ src, uint32_t* __restrict__ codes,
@@ -221,7 +223,8 @@ __device__ __forceinline__ uint32_t mx_put2(float lo, float hi) {
 
 // Rows of whole blocks, 16-byte aligned output.  A lane loads one word (eight codes) per
 // step; for 16-bit outputs it writes its own 16 bytes, for FP32 the words change hands inside
-// the warp so that each store instruction writes 512 consecutive bytes.  Bound by HBM.
+// the warp so that each store instruction writes 512 consecutive bytes.  Bound by HBM: 8192 x
+// 8192 to FP32 48.5 us (6.3 TB/s), 16384 x 8192 to BF16 55.5 (6.1).
 template <int T>
 __global__ void __launch_bounds__(256)
 mx_decode_kernel(const uint32_t* __restrict__ codes, const unsigned char* __restrict__ scales, void* __restrict__ dst,
@@ -271,7 +274,8 @@ mx_decode_kernel(const uint32_t* __restrict__ codes, const unsigned char* __rest
 
 // Any row length and alignment: a warp takes kMxRun consecutive pairs of blocks of a row, a lane two
 // consecutive elements (a byte) of each, so that its stores are consecutive; PAIRED: rows of
-// an even number of 16-bit elements, stored two at a time.
+// an even number of 16-bit elements, stored two at a time.  5001 x 2050 to FP16 11.4 us (one element
+// per lane 18.3).
 constexpr int kMxRun = 4;            // as many as mx_decode8 takes
 template <int T, bool PAIRED>
 __global__ void __launch_bounds__(256)

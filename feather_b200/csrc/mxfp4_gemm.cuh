@@ -19,6 +19,17 @@
 // multiplied (two accumulators alternate).  Every wait is bounded; a CTA that gave up
 // frees its tensor memory.
 //
+// What it took, at 16384 x 8192 x 4096 (NT = 224): one lane of the issuing warp walking the stages
+// by itself 382 us; the whole warp walking them (uniform addresses), one elected lane issuing 244;
+// the result through shared memory and tensor-map copies instead of 2-byte stores 219 us = 5.0
+// PFLOP/s in short runs.  Products alone, operands in place and nothing awaited, take 148 us;
+// a stage needs 90 bytes per clock from L2, and only four fit.  Under load the 1000 W cap holds the
+// SM at 1.43 GHz: 258 us, 4.3 PFLOP/s, 3.1 times the bf16 rate measured so.  Pairs of CTAs
+// (cta_group::2, 256 x 224 tiles, 30 KB instead of 44 per CTA and stage) took 249 .. 263 us and were
+// dropped; so was a split over clusters of eight (they do not all run at once).
+// Small: 2048 x 5632 x 33 6.8 us (four CTAs per tile; whole 8.1), 5001 x 2050 x 200 to FP32 10.6.
+// Memory-bound: 16384 x 16384 x 16 27 us (5.3 TB/s).
+//
 // Few tiles: a cluster of 2 or 4 CTAs shares one tile, each with its part of the row; the
 // partial sums meet through distributed shared memory and are added in rank order, each CTA
 // storing its share of the columns.  No scratch in global memory, the same bits every run.

@@ -11,26 +11,32 @@
 // vector is brought to FP16 block by block.
 //
 // Block-diagonal B.  The scales differ from row to row and block to block, so the sums of
-// different blocks must not meet before they are scaled.  A lane loads 16 bytes of a row: one
-// whole block.  The four lanes of a row hold four neighbouring blocks, and a product adds
-// over all four -- but it has eight columns: column 2 t and 2 t + 1 hold the vector for lane
-// t's block and zeros for the other three lanes' slots.  The accumulator that lane t gets
-// back for its row is then the sum of ITS block alone, so it multiplies it with its own scale,
-// and nothing moves between lanes until the row's end.  The two columns per block hold the
-// two halves of an FP32 vector, or two vectors.
+// different blocks must not meet before they are scaled.  A lane holds whole blocks of a row; the
+// four lanes of a row hold neighbouring ones, and a product adds over all four -- but it has
+// eight columns: two columns hold the vector for lane t's block (or blocks) and zeros for the
+// other three lanes' slots.  The accumulator that lane t gets back for its row is then the sum
+// of ITS block alone, so it multiplies it with its own scale, and nothing moves between lanes
+// until the row's end.
 //
 // The vector.  A block is scaled by a power of two so that its largest finite element lies in
-// [2^14, 2^15), and rounded to FP16: FP16, BF16 and packed values are exact (elements 2^-39 of
-// the block's largest and below lose bits that an FP32 sum would not keep either); FP32
-// values are split in two, x = hi + lo, each rounded to nearest, which leaves an error of at
-// most 2^-24 of the element -- one FP32 rounding.  The block sum (FP32) is multiplied by
-// the vector block's power of two and then, in an FMA, by the matrix block's.
+// [2^14, 2^15), and rounded to FP16.  FP16, BF16 and packed values are exact but for what lies
+// below FP16's smallest step, 2^-40 of the block's largest element -- less than the FP32 sum
+// keeps.  FP32 values are split in two, x = hi + lo, each rounded to nearest: at most 2^-24 of the
+// element (one FP32 rounding) or that same 2^-40.  The block sum (FP32) is multiplied by the
+// vector block's power of two and then, in an FMA, by the matrix block's.
 //
-// Work split.  A CTA per SM owns a range of 16-row groups; its 16 warps split the row's tiles of
-// 128 codes (and, for short rows, the groups): a warp keeps its range of columns for all
-// groups and leaves a partial sum per row in shared memory, so there is no barrier until
-// the CTA's rows are done; then the partials are added in warp order (same bits every run).
-// Loads go to registers, kMgDepth tiles of two groups ahead.
+// Two kernels.  mx_gemv_ring_kernel: one or two columns per block, any size (below).
+// mx_gemv_many_kernel: four or eight, for matrices that are too small to go to the tensor cores
+// as digits (mxfp4_gemm.cuh); a tile is 16 rows x 128 codes, loaded to registers two tiles ahead.
+//
+// Work split, both.  A CTA per SM owns a range of 16-row groups; its 16 warps split the row's
+// columns (and, for short rows, the groups): a warp keeps its range of columns for all groups and
+// leaves a partial sum per row in shared memory, so there is no barrier until the CTA's rows are
+// done; then the partials are added in warp order (same bits every run).
+//
+// Measured, one FP16 vector: 16384 x 16384 26.4 us (5.4 TB/s), 8192 x 8192 11.1, 32000 x 2048 9.8,
+// 2048 x 2048 3.1, 256 x 2048 3.0; FP32 at 16384 x 16384 31.8, two FP16 vectors 34.9.  The first
+// version (tiles of 16 x 128 loaded to registers, as the many-column kernel still does) took 43.4.
 #pragma once
 #include "attention_tc.cuh"   // tensor-map copies
 #include "gemv_common.cuh"
@@ -178,8 +184,10 @@ __device__ __forceinline__ void mg_stage(const MxGemvArgs& a, __half* vec, float
     }
 }
 
-// VT: type of the vector (kSrc...); COLS: columns, 1, 2, 4 or 8 (an FP32 vector takes two); R:
-// 16-row groups a warp multiplies with the same vector registers.
+// Four or eight columns.  A lane takes 16 bytes of a row, one block; columns 2 t and 2 t + 1 of a product
+// are two vectors, or the halves of an FP32 one, for lane t's block.  VT: type of the vector
+// (kSrc...); COLS: columns, an FP32 vector takes two; R: 16-row groups a warp multiplies with the
+// same vector registers.
 template <int VT, int COLS, int R>
 __global__ void __launch_bounds__(kMgThreads, 1)
 mx_gemv_many_kernel(const MxGemvArgs a) {
@@ -378,7 +386,8 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
 // lines), that it fills itself with tensor-map copies (128-byte swizzle: the reads below are free of
 // bank conflicts); it refills a slot as soon as it has read it, so nothing is shared and nothing
 // but arrival is waited for.  Loads straight to registers reached 3.9 TB/s at 16384 x 16384 (the
-// bytes in flight hang on the scoreboard), this 5.0.
+// bytes in flight hang on the scoreboard), this 5.4.  The vector is loaded before the first copies are
+// issued and staged while they travel: its loads behind 19 MB of copies had cost 3 us.
 constexpr int kMrRows = 16, kMrLines = 2, kMrSlotBytes = kMrRows * kMrLines * 128;
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
