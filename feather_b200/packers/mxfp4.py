@@ -43,8 +43,7 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
     if isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor):
         idx = codes.get_device()
         if (idx >= 0 and scales.get_device() == idx
-                and (codes.dtype is torch.uint8 or codes.dtype in _CODE_DTYPES)
-                and (scales.dtype is torch.uint8 or scales.dtype in _SCALE_DTYPES)
+                and codes.dtype in _CODE_DTYPES and scales.dtype in _SCALE_DTYPES
                 and codes.is_contiguous() and scales.is_contiguous()
                 and codes.numel() >= rows * blocks * BLOCK_BYTES and scales.numel() >= rows * blocks
                 and (blocks == 0 or not (codes.shape[-1] % (blocks * BLOCK_BYTES) or scales.shape[-1] % blocks))):
@@ -66,15 +65,10 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
     raise ValueError(f"{name}_codes and {name}_scales must be on the same device")
 
 
-def call(fn, idx: int, *args) -> None:
-    """``fn(*args, stream)`` with device ``idx`` current, on its current stream."""
-    if torch._C._cuda_getDevice() == idx:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
-    else:
-        with torch.cuda.device(idx):
-            status = fn(*args, _lib.current_stream_ptr(idx))
-    if status:
-        _lib.check(status)
+# The calls below launch on the current stream of their operands' device; with another device
+# current they make it current and start over, so that the usual case pays one comparison.
+current_device = torch._C._cuda_getDevice
+current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -95,16 +89,23 @@ def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         codes, scales = pack_mxfp4_tensor(x.cuda())
         return codes.cpu(), scales.cpu()
     lib = _lib.load()
+    device = x.device
+    idx = device.index
+    if current_device() != idx:
+        with torch.cuda.device(idx):
+            return pack_mxfp4_tensor(x)
     if not x.is_contiguous():
         x = x.contiguous()
     *lead, n = x.shape
     blocks = (n + BLOCK - 1) // BLOCK
-    device = x.device
     codes = torch.empty(*lead, blocks * BLOCK_BYTES, dtype=torch.uint8, device=device)
     scales = torch.empty(*lead, blocks, dtype=torch.uint8, device=device)
     total = x.numel()
     if total:
-        call(lib.feather_encode_mxfp4, device.index, x.data_ptr(), src, codes.data_ptr(), scales.data_ptr(), total // n, n)
+        status = lib.feather_encode_mxfp4(x.data_ptr(), src, codes.data_ptr(), scales.data_ptr(), total // n, n,
+                                          current_stream(idx))
+        if status:
+            _lib.check(status)
     return codes, scales
 
 
@@ -126,7 +127,13 @@ def unpack_mxfp4_tensor(codes: torch.Tensor, scales: torch.Tensor, n: int | None
         raise ValueError(f"n={n} does not have {blocks} blocks of {BLOCK}")
     rows = scales.numel() // blocks if blocks else 0
     idx = as_packed(codes, scales, rows, n, "m")
+    if current_device() != idx:
+        with torch.cuda.device(idx):
+            return unpack_mxfp4_tensor(codes, scales, n, dtype)
     out = torch.empty(*lead, n, dtype=dtype, device=codes.device)
     if rows:
-        call(_lib.load().feather_decode_mxfp4, idx, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows, n)
+        status = _lib.load().feather_decode_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dst, rows, n,
+                                                  current_stream(idx))
+        if status:
+            _lib.check(status)
     return out

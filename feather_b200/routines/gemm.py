@@ -12,7 +12,7 @@ import math
 import torch
 
 from .. import _lib
-from ..packers.mxfp4 import BLOCK_BYTES, as_packed, blocks_of, call, dtype_id
+from ..packers.mxfp4 import BLOCK_BYTES, as_packed, blocks_of, current_device, current_stream, dtype_id
 
 __all__ = ["gemv_mxfp4_acc_fp32_gpu", "gemm_mxfp4_acc_fp32_gpu"]
 
@@ -22,7 +22,7 @@ MAX_VECTORS = 64
 def _shape(m_shape) -> tuple[int, int]:
     if len(m_shape) != 2:
         raise ValueError("m_shape must be the unpacked (M, N) of the matrix")
-    M, N = map(int, m_shape)
+    M, N = int(m_shape[0]), int(m_shape[1])
     if M < 0 or N < 0:
         raise ValueError("m_shape must not be negative")
     return M, N
@@ -67,6 +67,9 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
         raise ValueError("v must be a CUDA tensor on the matrix's device")
     if batch > MAX_VECTORS:
         raise ValueError(f"at most {MAX_VECTORS} vectors: pack them and use gemm_mxfp4_acc_fp32_gpu")
+    if current_device() != idx:
+        with torch.cuda.device(idx):
+            return gemv_mxfp4_acc_fp32_gpu(m_codes, m_scales, v, m_shape, v_scales, out)
     if out is not None:
         _check_out(out, batch * M, torch.float32, v.device)
     elif dims == 1:
@@ -78,8 +81,10 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
         # one FP32 or two 16-bit vectors never need one
         need = 0 if batch == 1 or scales_ptr is not None else lib.feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype)
         ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
-        call(lib.feather_gemv_mxfp4, idx, m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr,
-             out.data_ptr(), ws.data_ptr() if need else None, M, N, batch)
+        status = lib.feather_gemv_mxfp4(m_codes.data_ptr(), m_scales.data_ptr(), v.data_ptr(), v_dtype, scales_ptr,
+                                        out.data_ptr(), ws.data_ptr() if need else None, M, N, batch, current_stream(idx))
+        if status:
+            _lib.check(status)
     return out
 
 
@@ -103,11 +108,16 @@ def gemm_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, x_cod
     batch = math.prod(lead)
     if as_packed(x_codes, x_scales, batch, N, "x") != idx:
         raise ValueError("m and x must be on the same device")
+    if current_device() != idx:
+        with torch.cuda.device(idx):
+            return gemm_mxfp4_acc_fp32_gpu(m_codes, m_scales, x_codes, x_scales, m_shape, out_dtype, out)
     if out is not None:
         _check_out(out, batch * M, out_dtype, x_codes.device)
     else:
         out = torch.empty(*lead, M, dtype=out_dtype, device=x_codes.device)
     if M and batch:
-        call(_lib.load().feather_gemm_mxfp4, idx, m_codes.data_ptr(), m_scales.data_ptr(), x_codes.data_ptr(),
-             x_scales.data_ptr(), out.data_ptr(), dst, M, N, batch)
+        status = _lib.load().feather_gemm_mxfp4(m_codes.data_ptr(), m_scales.data_ptr(), x_codes.data_ptr(),
+                                                x_scales.data_ptr(), out.data_ptr(), dst, M, N, batch, current_stream(idx))
+        if status:
+            _lib.check(status)
     return out

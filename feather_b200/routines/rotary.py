@@ -14,7 +14,7 @@ import torch
 
 from .. import _lib
 from ..packers.fp8 import _tag, as_words
-from ..packers.mxfp4 import call, dtype_id
+from ..packers.mxfp4 import current_device, current_stream, dtype_id
 
 __all__ = ["rotary_frequencies", "rotary_gpu"]
 
@@ -112,6 +112,9 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     total = tokens * heads * dim
     if last != 1 and total:
         raise ValueError("the last dimension of x must be contiguous")
+    if current_device() != idx:
+        with torch.cuda.device(idx):
+            return rotary_gpu(x, positions, inv_freq, layout, mode, scale, out)
     given = out is not None
     if mode is None:
         if not given:
@@ -125,7 +128,9 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
         if out.numel() != total // 4 or out.device != x.device:
             raise ValueError("out must hold heads * tokens * dim / 4 packed words on x's device")
     if total:
-        call(_lib.load().feather_rotary, idx, x.data_ptr(), dtype, token_stride, head_stride, positions.data_ptr(),
-             1 if wide else 0, inv_freq.data_ptr(), out.data_ptr(), out_mode, tokens, heads, dim, rotated, LAYOUTS[layout],
-             scale)
+        status = _lib.load().feather_rotary(x.data_ptr(), dtype, token_stride, head_stride, positions.data_ptr(),
+                                            1 if wide else 0, inv_freq.data_ptr(), out.data_ptr(), out_mode, tokens, heads,
+                                            dim, rotated, LAYOUTS[layout], scale, current_stream(idx))
+        if status:
+            _lib.check(status)
     return out if mode is None or given else _tag(out, mode)

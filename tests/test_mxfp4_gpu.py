@@ -455,7 +455,7 @@ def test_projections_rotation_and_attention_together():
 
 def test_captured_and_replayed_on_another_stream():
     M, N = 300, 512
-    w = packed(M, N, 1)
+    w, large = packed(M, N, 1), packed(3000, 8 * N, 2)
     x = torch.randn(4, N, device="cuda")
     inv, pos = fb.rotary_frequencies(60), torch.arange(4, device="cuda")
     stream = torch.cuda.Stream()
@@ -465,7 +465,8 @@ def test_captured_and_replayed_on_another_stream():
         a = fb.gemm_mxfp4_acc_fp32_gpu(*w, c, s, (M, N))
         b = fb.gemv_mxfp4_acc_fp32_gpu(*w, x, (M, N))
         r = fb.rotary_gpu(a.view(4, 5, 60), pos, inv)
-        return c, s, a, b, r, fb.unpack_mxfp4_tensor(c, s)
+        d = fb.gemv_mxfp4_acc_fp32_gpu(*large, x.repeat(1, 8), (3000, 8 * N))      # the digits' workspace is the graph's
+        return c, s, a, b, r, fb.unpack_mxfp4_tensor(c, s), d
     with torch.cuda.stream(stream):
         chain()
     stream.synchronize()
