@@ -866,46 +866,52 @@ static unsigned stream_grid(long long units, const DeviceInfo& dev) {
     return (unsigned)(ctas < 1 ? 1 : ctas < most ? ctas : most);
 }
 
+// A kernel that begins with in_turn(): its CTAs take the SMs as the kernel in front leaves them.
+template <typename K, typename... Args>
+static int launch_in_turn(K kernel, dim3 grid, int threads, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? launch_status() : FEATHER_ERR_LAUNCH;
+}
+
 template <int T>
 static int mx_encode_launch(const void* src, unsigned char* codes, unsigned char* scales, long long rows, long long cols,
                             const DeviceInfo& dev, cudaStream_t s) {
-    if (cols % kMxBlock == 0 && aligned(src, 16)) {
-        const long long words = rows * (cols / 8);
-        mx_encode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
-            src, reinterpret_cast<uint32_t*>(codes), scales, words);
-    } else {
-        typedef typename MxElem<T>::type E;
-        const uint32_t words_row = 4u * (uint32_t)mx_blocks(cols);
-        const long long words = rows * words_row;
-        const unsigned grid = stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev);
-        uint32_t* to = reinterpret_cast<uint32_t*>(codes);
-        if (sizeof(E) == 2 && cols % 2 == 0 && aligned(src, 4))
-            mx_encode_rows_kernel<T, 4><<<grid, 256, 0, s>>>(static_cast<const E*>(src), to, scales, words, cols, words_row);
-        else
-            mx_encode_rows_kernel<T, sizeof(E)><<<grid, 256, 0, s>>>(static_cast<const E*>(src), to, scales, words, cols, words_row);
-    }
-    return launch_status();
+    typedef typename MxElem<T>::type E;
+    const uint32_t words_row = 4u * (uint32_t)mx_blocks(cols);
+    const long long words = rows * words_row;
+    const dim3 grid(stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev));
+    uint32_t* to = reinterpret_cast<uint32_t*>(codes);
+    if (cols % kMxBlock == 0 && aligned(src, 16)) return launch_in_turn(mx_encode_kernel<T>, grid, 256, s, src, to, scales, words);
+    const E* from = static_cast<const E*>(src);
+    if (sizeof(E) == 2 && cols % 2 == 0 && aligned(src, 4))
+        return launch_in_turn(mx_encode_rows_kernel<T, 4>, grid, 256, s, from, to, scales, words, cols, words_row);
+    return launch_in_turn(mx_encode_rows_kernel<T, (int)sizeof(E)>, grid, 256, s, from, to, scales, words, cols, words_row);
 }
 
 template <int T>
 static int mx_decode_launch(const unsigned char* codes, const unsigned char* scales, void* dst, long long rows,
                             long long cols, const DeviceInfo& dev, cudaStream_t s) {
+    typedef typename MxElem<T>::type E;
     if (cols % kMxBlock == 0 && aligned(dst, 16)) {
         const long long words = rows * (cols / 8);
-        mx_decode_kernel<T><<<stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev), 256, 0, s>>>(
-            reinterpret_cast<const uint32_t*>(codes), scales, dst, words);
-    } else {
-        typedef typename MxElem<T>::type E;
-        const int blocks = mx_blocks(cols), runs = (blocks + 2 * kMxRun - 1) / (2 * kMxRun);
-        const unsigned grid = stream_grid(rows * runs, dev);
-        bool paired = false;
-        if constexpr (sizeof(E) == 2) {
-            paired = cols % 2 == 0 && aligned(dst, 4);
-            if (paired) mx_decode_rows_kernel<T, true><<<grid, 256, 0, s>>>(codes, scales, static_cast<E*>(dst), rows, cols, blocks, runs);
-        }
-        if (!paired) mx_decode_rows_kernel<T, false><<<grid, 256, 0, s>>>(codes, scales, static_cast<E*>(dst), rows, cols, blocks, runs);
+        const dim3 grid(stream_grid((words + 32 * kMxSteps - 1) / (32 * kMxSteps), dev));
+        return launch_in_turn(mx_decode_kernel<T>, grid, 256, s, reinterpret_cast<const uint32_t*>(codes), scales, dst, words);
     }
-    return launch_status();
+    const int blocks = mx_blocks(cols), runs = (blocks + 2 * kMxRun - 1) / (2 * kMxRun);
+    const dim3 grid(stream_grid(rows * runs, dev));
+    E* to = static_cast<E*>(dst);
+    if constexpr (sizeof(E) == 2)
+        if (cols % 2 == 0 && aligned(dst, 4))
+            return launch_in_turn(mx_decode_rows_kernel<T, true>, grid, 256, s, codes, scales, to, rows, cols, blocks, runs);
+    return launch_in_turn(mx_decode_rows_kernel<T, false>, grid, 256, s, codes, scales, to, rows, cols, blocks, runs);
 }
 
 template <int VT, int COLS>
@@ -1099,18 +1105,9 @@ static int mx_gemv_digits(const MxGemvArgs& v, int batch, unsigned char* workspa
         a.x_scales = scales;
         a.batch = nv * kGmDigits;
         a.align = mx_scale_align(a.m_scales, scales, a.blocks);
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)((4ll * v.blocks * nv + 255) / 256));
-        cfg.blockDim = dim3(256);
-        cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (cudaLaunchKernelEx(&cfg, mx_digits_kernel<VT>, a.v, reinterpret_cast<uint32_t*>(workspace), scales,
-                               (long long)v.N, v.blocks, nv) != cudaSuccess)
-            return FEATHER_ERR_LAUNCH;
+        if (int st = launch_in_turn(mx_digits_kernel<VT>, dim3((unsigned)((4ll * v.blocks * nv + 255) / 256)), 256, s, a.v,
+                                    reinterpret_cast<uint32_t*>(workspace), scales, (long long)v.N, v.blocks, nv))
+            return st;
         const int st = nv == 1   ? mx_gemm_launch<16, kSrcF32, true>(workspace, a, dev, s)
                        : nv == 2 ? mx_gemm_launch<32, kSrcF32, true>(workspace, a, dev, s)
                        : nv <= 4 ? mx_gemm_launch<48, kSrcF32, true>(workspace, a, dev, s)
@@ -1153,10 +1150,9 @@ static int rotary_launch(RotaryArgs a, const DeviceInfo& dev, cudaStream_t s) {
     gy = (items + per - 1) / per;
     a.items_each = (int)per;
     const dim3 grid((unsigned)gx, (unsigned)gy);
-    if (v == kWide) rotary_kernel<T, MODE, kWide><<<grid, kRotThreads, 0, s>>>(a);
-    else if (v == 4) rotary_kernel<T, MODE, 4><<<grid, kRotThreads, 0, s>>>(a);
-    else rotary_kernel<T, MODE, 1><<<grid, kRotThreads, 0, s>>>(a);
-    return launch_status();
+    return v == kWide ? launch_in_turn(rotary_kernel<T, MODE, kWide>, grid, kRotThreads, s, a)
+           : v == 4   ? launch_in_turn(rotary_kernel<T, MODE, 4>, grid, kRotThreads, s, a)
+                      : launch_in_turn(rotary_kernel<T, MODE, 1>, grid, kRotThreads, s, a);
 }
 
 template <int T>

@@ -79,6 +79,13 @@ __device__ __forceinline__ void mx_decode8(uint32_t w, uint32_t (&h)[4]) {
         : "r"(w));
 }
 
+// First thing in a kernel launched ahead of its turn (programmatic stream serialisation): lets
+// the next kernel do the same, and waits for the one in front before memory is touched.
+__device__ __forceinline__ void in_turn() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // The largest |x| of eight values as an FP32 bit pattern, and the values.
 template <int T>
 __device__ __forceinline__ uint32_t mx_load8(const void* src, long long e, float (&x)[8]) {
@@ -118,6 +125,7 @@ template <int T>
 __global__ void __launch_bounds__(256)
 mx_encode_kernel(const void* __restrict__ src, uint32_t* __restrict__ codes, unsigned char* __restrict__ scales,
                  long long n_words) {
+    in_turn();
     const int lane = threadIdx.x & 31;
     const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
     const long long warp = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -163,6 +171,7 @@ template <int T, int W>
 __global__ void __launch_bounds__(256)
 mx_encode_rows_kernel(const typename MxElem<T>::type* __restrict__ src, uint32_t* __restrict__ codes,
                       unsigned char* __restrict__ scales, long long n_words, long long cols, uint32_t words_row) {
+    in_turn();
     const int lane = threadIdx.x & 31;
     const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
     const long long warp = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -229,6 +238,7 @@ template <int T>
 __global__ void __launch_bounds__(256)
 mx_decode_kernel(const uint32_t* __restrict__ codes, const unsigned char* __restrict__ scales, void* __restrict__ dst,
                  long long n_words) {
+    in_turn();
     const int lane = threadIdx.x & 31;
     const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
     const long long warp = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -282,6 +292,7 @@ __global__ void __launch_bounds__(256)
 mx_decode_rows_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
                       typename MxElem<T>::type* __restrict__ dst, long long rows, long long cols, int blocks_row,
                       int runs_row) {
+    in_turn();
     const int lane = threadIdx.x & 31;
     const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, runs = rows * runs_row;
     for (long long run = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; run < runs; run += warps) {

@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kRotThreads, 4)
 rotary_kernel(const RotaryArgs a) {
     typedef typename MxElem<T>::type E;
     __shared__ float2 turns[kRotAngles];
+    in_turn();
     const int half = a.rotated / 2;
     const int turned = half / V;                                   // items of a head that turn
     const int still = (a.dim - a.rotated + 2 * V - 1) / (2 * V);   // items that pass through

@@ -40,8 +40,8 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
 
     ``m_codes``, ``m_scales``: what ``pack_mxfp4_tensor`` returns for an ``(M, N)`` matrix.
     ``v``: a contiguous float16, bfloat16 or float32 tensor of shape ``(N,)`` or ``(batch, N)``, or
-    packed codes together with ``v_scales``.  Eight vectors (four float32 ones) go through one
-    pass over the matrix; at most 64."""
+    packed codes together with ``v_scales``.  Up to eight vectors go through one pass over the
+    matrix (four float32 ones where it is small); at most 64."""
     M, N = _shape(m_shape)
     idx = as_packed(m_codes, m_scales, M, N, "m")
     if not isinstance(v, torch.Tensor):

@@ -533,8 +533,8 @@ int feather_decode_mxfp4(const uint8_t* codes, const uint8_t* scales, void* dst,
 
 /*
  * out[b][r] = sum_j value(m[r][j]) * v[b][j]: a packed MXFP4 matrix times
- * 0 <= batch <= 64 vectors, FP32 accumulation, eight vectors (four FP32 ones)
- * per pass over the matrix.  No counterpart in the reference.
+ * 0 <= batch <= 64 vectors, FP32 accumulation, up to eight vectors per pass over
+ * the matrix (four FP32 ones where it is small).  No counterpart in the reference.
  *   v         batch x N values of v_dtype, contiguous, or FEATHER_SRC_MXFP4:
  *             packed codes with v_scales (ignored otherwise)
  *   out       batch x M floats
