@@ -34,8 +34,8 @@
 // leaves a partial sum per row in shared memory, so there is no barrier until the CTA's rows are
 // done; then the partials are added in warp order (same bits every run).
 //
-// Measured, one FP16 vector: 16384 x 16384 26.4 us (5.4 TB/s), 8192 x 8192 11.1, 32000 x 2048 9.8,
-// 2048 x 2048 3.1, 256 x 2048 3.0; FP32 at 16384 x 16384 31.8, two FP16 vectors 34.9.  The first
+// Measured, one FP16 vector: 16384 x 16384 26.0 us (5.5 TB/s), 8192 x 8192 10.2, 32000 x 2048 9.1,
+// 4096 x 4096 4.6, 256 x 2048 3.0; FP32 at 16384 x 16384 31.5, two FP16 vectors 34.9.  The first
 // version (tiles of 16 x 128 loaded to registers, as the many-column kernel still does) took 43.4.
 #pragma once
 #include "attention_tc.cuh"   // tensor-map copies
@@ -386,13 +386,22 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
 // lines), that it fills itself with tensor-map copies (128-byte swizzle: the reads below are free of
 // bank conflicts); it refills a slot as soon as it has read it, so nothing is shared and nothing
 // but arrival is waited for.  Loads straight to registers reached 3.9 TB/s at 16384 x 16384 (the
-// bytes in flight hang on the scoreboard), this 5.4.  The vector is loaded before the first copies are
+// bytes in flight hang on the scoreboard), this 5.5.  The vector is loaded before the first copies are
 // issued and staged while they travel: its loads behind 19 MB of copies had cost 3 us.
 constexpr int kMrRows = 16, kMrLines = 2, kMrSlotBytes = kMrRows * kMrLines * 128;
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// The same boxes into L2 only.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
 }
 // Host side: rows of whole lines as {128 bytes, rows, lines} with boxes of 16 rows x 2 lines.
 inline bool mr_make_map(CUtensorMap* map, const void* base, long long row_bytes, long long rows) {
@@ -444,6 +453,24 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
 
     const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
     const int wk = a.col_warps, wr = kMgWarps / wk, my_k = warp & (wk - 1), my_r = warp / wk;
+    // Ask L2 for the first slots' codes while the kernel in front still runs: harmless whatever it
+    // writes, because its writes land in L2 too.  (8192 x 8192 11.2 -> 10.2 us, 16384 x 16384 26.9 ->
+    // 26.0, 256 x 2048 the same.)
+    if (lane == 0 && my_r < tasks) {
+        const int n_blk = min(a.chunk_blocks, a.blocks), spans = (n_blk + 8 * kMrLines - 1) / (8 * kMrLines);
+        const int from = spans * my_k / wk, n = spans * (my_k + 1) / wk - from;
+        int span = 0, task = my_r;
+        for (int i = 0; i < SLOTS && task < min(a.slots, tasks) && n > 0; ++i) {
+            const int y = (g_begin + task) * kMrRows, z = (from + span) * kMrLines;
+            if constexpr (WHOLE) {
+                tma_prefetch_3d(&map, 0, y, z);
+            } else {
+#pragma unroll
+                for (int l = 0; l < kMrLines; ++l) tma_prefetch_2d(&map, (z + l) * 128, y);
+            }
+            if (++span == n) span = 0, task += wr;
+        }
+    }
     __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     bool ok = true;
