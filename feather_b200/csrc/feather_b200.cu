@@ -1063,7 +1063,7 @@ static int mx_scale_align(const void* m_scales, const void* x_scales, int blocks
 // 4096^2 x 8 14.8 / 12.1, x 3 9.4 / 10.2, 2048^2 x 8 6.7 / 9.0, 256 x 2048 x 8 6.6 / 9.0.
 static bool mx_wants_digits(long long M, long long N, int batch, int v_dtype) {
     const long long cols = (long long)batch * (v_dtype == FEATHER_SRC_F32 ? 2 : 1);
-    return cols > 2 && cols * M * N >= (80ll << 20);
+    return cols > 2 && N > 0 && M >= (((80ll << 20) + cols - 1) / cols + N - 1) / N;   // cols M N >= 80 M
 }
 
 // Tiles of 224 or of 128 rows of x: those whose waves take less, a wave of the wide ones taking
@@ -1778,7 +1778,7 @@ int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const vo
     if (v_dtype < 0 || v_dtype > FEATHER_SRC_MXFP4) return FEATHER_ERR_MODE;
     if (M == 0 || batch == 0) return FEATHER_OK;
     if (!out) return FEATHER_ERR_BAD_ARG;
-    if (N > kMxMaxCols || M > kMxMaxRows || batch > 64) return FEATHER_ERR_TOO_LARGE;
+    if (N > kMxMaxCols || M > kMxMaxRows - 128 || batch > 64) return FEATHER_ERR_TOO_LARGE;
     if (!aligned(out, 4)) return FEATHER_ERR_MISALIGNED;
     const bool packed = v_dtype == FEATHER_SRC_MXFP4;
     if (N > 0) {

@@ -148,3 +148,18 @@ def test_angle_reduction_is_good_to_a_tenth_of_a_millionth():
     # angle error: |p f| 2^-52 from the 64-bit products, half an ulp of a fraction below 1/2 (2^-26) times 2 pi
     bound = (p * f) * 2.0 ** -51 + 2 * math.pi * 2.0 ** -26
     assert bool(((got - torch.sin(p * f)).abs() <= bound).all())
+
+
+def test_sizes_at_the_end_of_their_range(lib):
+    p, big = 4096, 1 << 31
+    assert lib.feather_gemv_mxfp4(p, p, p, 0, None, p, None, big - 127, 8, 1, None) == -8      # rows are counted in 32 bits
+    assert lib.feather_gemv_mxfp4(p, p, p, 3, p, p, None, big, 8, 2, None) == -8
+    # digits from columns x M x N = 80 M on, without passing 64 bits on the way; FP32 vectors are two columns each
+    need = lib.feather_gemv_mxfp4_workspace_bytes
+    assert need((1 << 62) + 1, 1 << 30, 64, 1) == need(1 << 20, 1 << 30, 8, 1) == 8 * 12 * (1 << 25) * 17
+    for vectors, dtype in ((3, 0), (2, 1), (64, 2)):
+        cols = vectors * (2 if dtype == 1 else 1)
+        for n in (1, 33, 4096):
+            m = -(-(80 << 20) // (cols * n))
+            assert need(m, n, vectors, dtype) > 0 and need(m - 1, n, vectors, dtype) == 0
+    assert need(100, 0, 64, 1) == 0 and need(1 << 40, 4096, 2, 0) == 0
