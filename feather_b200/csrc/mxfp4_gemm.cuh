@@ -191,7 +191,7 @@ constexpr int kGmDigits = 12;
 // n after d rows.  Four threads per block, eight elements each; the remainder is exact in FP32 (an
 // element and its code's value are within a factor of two, or the code is zero).  A row leaves at
 // most a quarter of the block's largest remainder, so after all of them 2^-24 of its largest
-// element is left: one FP32 rounding of that.  (16 rows: 39.6 us for 8 vectors at 16384 x
+// element is left: one FP32 rounding of that (or 2^-129, a quarter of the smallest scale).  (16 rows: 39.6 us for 8 vectors at 16384 x
 // 16384, 12 rows 38.8, before other steps.)  A block with an infinity or a NaN gets scale 255 in row 0.
 template <int VT>
 __global__ void __launch_bounds__(256)
@@ -276,8 +276,10 @@ __device__ __forceinline__ float gm_not_finite(const MxGemmArgs& g, int m, int n
     const unsigned char* s = g.x_scales + (long long)n * kGmDigits * g.blocks;
     float sum = 0.f;
     for (int b = 0; b < g.blocks; ++b) {
+        const uint32_t ms = g.m_scales[(long long)m * g.blocks + b];
+        if (ms == 255u) return __uint_as_float(0x7FC00000u);     // the row is NaN whatever the vector holds
         if (s[b] != 255) continue;
-        const float scale = mx_scale_value(g.m_scales[(long long)m * g.blocks + b]);
+        const float scale = mx_scale_value(ms);
         for (int i = 0; i < kMxBlock && (long long)b * kMxBlock + i < g.N; ++i) {
             const long long e = n * g.N + (long long)b * kMxBlock + i;
             const float v = g.v_dtype == kSrcF32   ? reinterpret_cast<const float*>(g.v)[e]
@@ -376,6 +378,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
                     tma_load_2d(at + L::kA, &map_x, (k_begin + k) * kGmBox, x0, full(s));
                 }
             }
+            // whoever gave up: shared memory outlives what was asked for
+            for (int i = max(it - L::kStages, 0); i < it; ++i)
+                mbar_wait(full(i % L::kStages), (uint32_t)((i / L::kStages) & 1), g.status);
         }
         __syncwarp();
     } else if (warp == 1) {

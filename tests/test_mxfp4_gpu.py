@@ -265,6 +265,46 @@ def test_gemv_values_that_are_not_finite_and_far_scales(dtype):
     assert bool(((got - v2.double() @ m.T).abs() <= gemv_bound(m, v2.double(), dtype == "fp32")).all())
 
 
+@pytest.mark.parametrize("vector", ["bf16", "fp32", "mxfp4"])
+@pytest.mark.parametrize("M,N,batch", [(40, 256, 1), (40, 300, 1), (40, 256, 2), (40, 256, 5), (9000, 4096, 3)])
+@pytest.mark.parametrize("up", [126, -120])
+def test_gemv_large_values_times_small_scales_and_the_reverse(M, N, batch, vector, up):
+    # sums over unscaled codes leave FP32's range, the results (around 2^60 or 2^-20) do not
+    kind = DTYPES.get(vector, torch.float32)
+    v = (values(batch, N, 2, torch.float32, spread=0.0).clamp(-2, 2) * 2.0 ** up).double()
+    codes, scales = O.quantise(values(M, N, 3, spread=0.0).double() * 2.0 ** (-60 if up > 0 else 100))
+    if vector == "mxfp4":
+        v, v_scales = O.quantise(v)
+        wide = O.dequantise(v, v_scales, N)
+    else:
+        v, v_scales = v.to(kind), None
+        wide = v.double()
+    m = O.dequantise(codes, scales, N)
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N), v_scales=v_scales).double()
+    if vector == "mxfp4" and batch > 1:
+        bound = gemm_bound(m, wide, torch.float32)
+    else:
+        # digits end at the smallest scale's half code: what is left of an element may also be 2^-129
+        bound = gemv_bound(m, wide, vector == "fp32") if M < 9000 else \
+            digits_bound(m, wide) + 2.0 ** -129 * m.abs().sum(1)
+    assert bool(((got - wide @ m.T).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_several_vectors_infinite_where_the_matrix_is_nan_elsewhere(dtype):
+    M, N = 9000, 4096
+    codes, scales = packed(M, N, 1)
+    scales = scales.clone()
+    scales[5, 7] = 255                                # a NaN block the infinity does not meet
+    scales[77, 2] = 255                               # one that it does
+    v = values(3, N, 2, DTYPES[dtype], spread=1.0)
+    v[1, 70] = float("inf")
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N)).double()
+    want = v.double() @ O.dequantise(codes, scales, N).T
+    assert torch.equal(got.isnan(), want.isnan()) and bool(want[1, 5].isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+
+
 # -------------------------------------------------------------------- gemm --
 def gemm_bound(m, x, dtype):
     """Per element: N / 64 products in a row add into one FP32 sum, each may lose 2^-22 of the products' size so far (the
