@@ -118,8 +118,8 @@ __device__ __forceinline__ uint32_t mx_load8(const void* src, long long e, float
 // Rows of whole blocks, 16-byte aligned: the matrix is a flat run of blocks.  Four threads
 // take a block, eight elements each (16- or 2 x 16-byte loads), and agree on the block's
 // maximum with two shuffles; a warp takes kMxSteps runs of 256 elements per trip.  Bound by
-// HBM: it reads every element once and writes 17/32 byte for each; 16384 x 8192 FP16 57.2 us
-// (5.9 TB/s).
+// HBM: it reads every element once and writes 17/32 byte for each; 16384 x 8192 FP16 56.7 us
+// (6.0 TB/s).
 constexpr int kMxSteps = 4;
 template <int T>
 __global__ void __launch_bounds__(256)
@@ -233,7 +233,7 @@ __device__ __forceinline__ uint32_t mx_put2(float lo, float hi) {
 // Rows of whole blocks, 16-byte aligned output.  A lane loads one word (eight codes) per
 // step; for 16-bit outputs it writes its own 16 bytes, for FP32 the words change hands inside
 // the warp so that each store instruction writes 512 consecutive bytes.  Bound by HBM: 8192 x
-// 8192 to FP32 48.5 us (6.3 TB/s), 16384 x 8192 to BF16 55.5 (6.1).
+// 8192 to FP32 48.2 us (6.3 TB/s), 16384 x 8192 to BF16 55.0 (6.2).
 template <int T>
 __global__ void __launch_bounds__(256)
 mx_decode_kernel(const uint32_t* __restrict__ codes, const unsigned char* __restrict__ scales, void* __restrict__ dst,

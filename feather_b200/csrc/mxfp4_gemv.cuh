@@ -35,7 +35,7 @@
 // done; then the partials are added in warp order (same bits every run).
 //
 // Measured, one FP16 vector: 16384 x 16384 26.0 us (5.5 TB/s), 8192 x 8192 10.2, 32000 x 2048 9.1,
-// 4096 x 4096 4.6, 256 x 2048 3.0; FP32 at 16384 x 16384 31.5, two FP16 vectors 34.9.  The first
+// 4096 x 4096 4.6, 256 x 2048 3.0; FP32 at 16384 x 16384 31.7, two FP16 vectors 34.5.  The first
 // version (tiles of 16 x 128 loaded to registers, as the many-column kernel still does) took 43.4.
 #pragma once
 #include "attention_tc.cuh"   // tensor-map copies
