@@ -20,8 +20,9 @@ __all__ = ["pack_mxfp4_tensor", "unpack_mxfp4_tensor"]
 BLOCK = 32
 BLOCK_BYTES = 16
 DTYPE_IDS = {torch.float16: _lib.SRC_F16, torch.float32: _lib.SRC_F32, torch.bfloat16: _lib.SRC_BF16}
+# bytes, and torch's own names for them where it has them
 _CODE_DTYPES = tuple(d for d in (torch.uint8, getattr(torch, "float4_e2m1fn_x2", None)) if d is not None)
-_SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
+_SCALE_DTYPES = tuple(d for d in (torch.uint8, getattr(torch, "float8_e8m0fnu", None)) if d is not None)
 
 
 def blocks_of(n: int) -> int:
@@ -67,8 +68,8 @@ def as_packed(codes: torch.Tensor, scales: torch.Tensor, rows: int, n: int, name
 
 # The calls below launch on the current stream of their operands' device; with another device
 # current they make it current and start over, so that the usual case pays one comparison.
-current_device = torch._C._cuda_getDevice
-current_stream = torch._C._cuda_getCurrentRawStream
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.current_stream_ptr)
 
 
 def pack_mxfp4_tensor(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,12 +1,17 @@
 """Microscaled 4-bit operators and rotary positions, host side: the oracle against the formats'
 definition, refusals of the C ABI and of the Python surface, the frequency tables.  No GPU."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import feather_b200 as fb
 from oracle import mxfp4_oracle as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -163,3 +168,21 @@ def test_sizes_at_the_end_of_their_range(lib):
             m = -(-(80 << 20) // (cols * n))
             assert need(m, n, vectors, dtype) > 0 and need(m - 1, n, vectors, dtype) == 0
     assert need(100, 0, 64, 1) == 0 and need(1 << 40, 4096, 2, 0) == 0
+
+
+@pytest.mark.parametrize("gone", ["torch.float8_e8m0fnu", "torch.float4_e2m1fn_x2", "torch._C._cuda_getDevice", "torch._C._cuda_getCurrentRawStream"])
+def test_import_without_what_not_every_torch_has(gone):
+    # a type or a private accessor that another torch lacks: the package imports, with the public calls in its place
+    code = f"""
+import torch
+if hasattr({gone.rpartition('.')[0]}, {gone.rpartition('.')[2]!r}):
+    del {gone}
+import feather_b200 as fb, feather_b200._lib as lib, feather_b200.packers.mxfp4 as mx
+assert fb.pack_fp8_tensor and torch.uint8 in mx._CODE_DTYPES and torch.uint8 in mx._SCALE_DTYPES
+if {gone!r}.endswith("getDevice"):
+    assert mx.current_device is torch.cuda.current_device
+if {gone!r}.endswith("RawStream"):
+    assert mx.current_stream is lib.current_stream_ptr
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert done.returncode == 0, done.stderr
