@@ -47,7 +47,9 @@ class PackedFP8(torch.Tensor):
 
 
 def _tag(words: torch.Tensor, mode: str) -> torch.Tensor:
-    t = words.as_subclass(PackedFP8)
+    """``words`` with the mode they hold now: a PackedFP8 keeps its identity and changes its tag
+    (a caller's buffer that held the other mode), another tensor comes back as a tagged alias."""
+    t = words if isinstance(words, PackedFP8) else words.as_subclass(PackedFP8)
     t.feather_mode = mode
     return t
 

@@ -84,7 +84,8 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
 
     Returns ``(tokens, heads, dim)`` of ``x``'s type (``out`` may be ``x`` itself where it is
     contiguous), or with ``mode`` "E5M2" / "E4M3" the FP8 words ``(heads, tokens, dim / 4)``: one
-    head's ``result[h]`` is a packed (tokens, dim) matrix.  The angles are computed in 64 bits, so
+    head's ``result[h]`` is a packed (tokens, dim) matrix.  Words written to ``out`` come back tagged with
+    ``mode`` too, and an ``out`` that carries a tag has it changed.  The angles are computed in 64 bits, so
     positions far into a context lose nothing."""
     if not (isinstance(x, torch.Tensor) and isinstance(positions, torch.Tensor) and isinstance(inv_freq, torch.Tensor)):
         raise TypeError("x, positions and inv_freq must be torch.Tensors")
@@ -115,13 +116,12 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
     if current_device() != idx:
         with torch.cuda.device(idx):
             return rotary_gpu(x, positions, inv_freq, layout, mode, scale, out)
-    given = out is not None
     if mode is None:
-        if not given:
+        if out is None:
             out = torch.empty(tokens, heads, dim, dtype=x.dtype, device=x.device)
         elif out.dtype != x.dtype or out.numel() != total or out.device != x.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor of x's type and size on its device")
-    elif not given:
+    elif out is None:
         out = torch.empty(heads, tokens, dim // 4, dtype=torch.uint32, device=x.device)
     else:
         out = as_words(out, "out")
@@ -133,4 +133,4 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                                             dim, rotated, LAYOUTS[layout], scale, current_stream(idx))
         if status:
             _lib.check(status)
-    return out if mode is None or given else _tag(out, mode)
+    return out if mode is None else _tag(out, mode)

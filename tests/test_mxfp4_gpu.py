@@ -441,6 +441,25 @@ def test_rotary_packs_every_pattern_like_the_packer(dtype, mode):
     assert torch.equal(got[~nan], want[~nan]) and torch.equal(got[nan] & 127, want[nan] & 127)
 
 
+def test_rotary_words_in_a_buffer_carry_their_mode():
+    # one buffer for both modes, tagged, untagged and typed otherwise: the calls that go by the tag decode what it holds now
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(6, 2, 64, generator=gen, device="cuda")
+    pos, inv = torch.arange(6, device="cuda"), fb.rotary_frequencies(64)
+    ones = {m: fb.pack_fp8_tensor(torch.ones(64, device="cuda"), m) for m in ("E5M2", "E4M3")}
+    tagged = fb.rotary_gpu(x, pos, inv, mode="E5M2")
+    for buffer in (tagged, torch.empty(2, 6, 16, dtype=torch.uint32, device="cuda"), torch.empty(2 * 6 * 16, dtype=torch.int32, device="cuda")):
+        for mode in ("E4M3", "E5M2", "E4M3"):
+            fresh = fb.rotary_gpu(x, pos, inv, mode=mode)
+            got = fb.rotary_gpu(x, pos, inv, mode=mode, out=buffer)
+            assert got.data_ptr() == buffer.data_ptr() and got.feather_mode == mode
+            assert torch.equal(got.as_subclass(torch.Tensor).flatten().view(torch.int32), fresh.as_subclass(torch.Tensor).flatten().view(torch.int32))
+            words = got.view(2, 96)[0]
+            assert torch.equal(fb.gemv(words, ones[mode].as_subclass(torch.Tensor), (6, 64)), fb.gemv(fresh[0], ones[mode], (6, 64)))
+            if buffer is tagged:
+                assert got is buffer and tagged.feather_mode == mode
+
+
 def test_rotary_strides_and_padding_rows_left_alone():
     gen = torch.Generator(device="cuda").manual_seed(1)
     qkv = torch.randn(9, 3, 4, 64, generator=gen, device="cuda", dtype=torch.float16)
