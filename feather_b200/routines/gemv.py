@@ -44,16 +44,17 @@ def gemv_fp8_ret_packed_gpu(m: torch.Tensor, v: torch.Tensor, m_shape, mode: str
     the result goes through the CPU packer, feather/packers/fp8.py:260-281).
 
     Returns ``ceil(M / 4)`` packed words (a ``PackedFP8`` tagged ``out_mode``,
-    default: ``mode``).  Small and mid-size matrices encode in the GEMV kernel's
+    default: ``mode``; ``out`` as it is, but for a tag of another mode, which is
+    changed).  Small and mid-size matrices encode in the GEMV kernel's
     epilogue; large ones (and rows that are not whole 16-byte chunks) run the
     encoder behind the GEMV kernel on ``workspace`` (M floats, allocated here
     when not given)."""
-    from ..packers.fp8 import _tag
+    from ..packers.fp8 import PackedFP8, _tag
     out_mode = mode if out_mode is None else out_mode
     with torch._C.DisableTorchFunctionSubclass():
         words = _gemv(m, v, m_shape, mode, out, 1 if static_matrix else 0,
                       out_mode_id=_lib.mode_id(out_mode), workspace=workspace)
-        return words if out is not None else _tag(words, out_mode)
+        return _tag(words, out_mode) if out is None or isinstance(out, PackedFP8) else words
 
 
 def gemv_fp8_multi_acc_fp32_gpu(m: torch.Tensor, v: torch.Tensor, m_shape, mode: str = "E5M2",

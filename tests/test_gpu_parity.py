@@ -872,6 +872,23 @@ def test_gemv_packed_output_feeds_next_gemv_and_rejects(fb):
     torch.cuda.synchronize()
 
 
+def test_gemv_packed_output_into_a_buffer_of_the_other_mode(fb):
+    """A tagged buffer that held the other format carries the new one's tag, so the
+    calls that go by the tag decode what it holds; an untagged one stays as it is."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    A = (0.05 * torch.randn(512, 512, device="cuda", generator=gen)).to(torch.float16)
+    x = torch.randn(512, device="cuda", generator=gen, dtype=torch.float16)
+    ops = {m: (fb.pack_fp8_tensor(A, m), fb.pack_fp8_tensor(x, m)) for m in ("E5M2", "E4M3")}
+    buf = fb.gemv_fp8_ret_packed_gpu(*ops["E5M2"], A.shape, "E5M2")
+    for mode in ("E4M3", "E5M2", "E4M3"):
+        assert fb.gemv_fp8_ret_packed_gpu(*ops[mode], A.shape, mode, out=buf) is buf
+        fresh = fb.gemv_fp8_ret_packed_gpu(*ops[mode], A.shape, mode)
+        assert buf.feather_mode == mode and torch.equal(buf.view(torch.int32), fresh.view(torch.int32))
+        assert torch.equal(fb.dot(buf, buf), fb.dot(fresh, fresh))
+    plain = torch.empty(128, dtype=torch.uint32, device="cuda")
+    assert fb.gemv_fp8_ret_packed_gpu(*ops["E4M3"], A.shape, "E4M3", out=plain) is plain
+
+
 # ------------------------------------------------------------ ReLU on unpack --
 @pytest.mark.parametrize("mode", MODES)
 def test_relu_all_codes_ragged_and_large_vs_oracle(fb, golden, mode):
