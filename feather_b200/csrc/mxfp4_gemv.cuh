@@ -64,17 +64,26 @@ __device__ __forceinline__ float2 mx_scale_pair(uint32_t s) {
     return make_float2(__uint_as_float(d << 16), __uint_as_float(d & 0xFFFF0000u));
 }
 
-// c x sv x sw, added to `sum`.  Both factors are powers of two, so the order changes nothing but what
-// leaves FP32's range on the way: the smaller factor first, a finite result never passes through an
-// infinity (2^124 in the vector against 2^-60 in the matrix) or loses bits as a subnormal.  FP16
-// vectors cannot: c x sv is below 2^25.  The ring kernel asks only vectors with such blocks to pay:
-// FP32 at 16384 x 16384 31.7 us, ordered throughout 33.1, never 31.5.
+// c x sv x sw, added to `sum`; both factors are powers of two.  c is a multiple of 2^-25 below 2^23 (of
+// a packed vector a multiple of 1/4), so c x sv is exact for 2^-124 <= sv < 2^100 (for a packed one below,
+// too), and always for FP16 vectors.  A vector with a block outside of that (`far`) has the factors
+// taken in the order in which nothing leaves FP32's range but what the result leaves it with:
+//   the larger first while it is at most 2^100: no overflow, and no bits lost below 2^-149;
+//   else their product, if the smaller one is below 1 (2^-27 .. 2^127, exact);
+//   else the smaller first.
+// (2^124 in the vector against 2^-60 in the matrix, 2^-149 against 2^127.)  Only such vectors pay:
+// FP32 at 16384 x 16384 31.7 us, some such order throughout 33.1, never 31.5.
 template <int VT>
-__device__ __forceinline__ float mx_scaled(float c, float sv, float sw, float sum) {
-    if constexpr (VT == kSrcF16) return fmaf(c * sv, sw, sum);
-    float first, second;                             // a NaN scale stays one
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(first) : "f"(sv), "f"(sw));
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(second) : "f"(sv), "f"(sw));
+__device__ __forceinline__ float mx_scaled(float c, float sv, float sw, float sum, bool far) {
+    if (VT == kSrcF16 || !far) return fmaf(c * sv, sw, sum);
+    float low, high;                                 // a NaN scale stays one
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(sv), "f"(sw));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(high) : "f"(sv), "f"(sw));
+    float first = high, second = low;
+    if (!(high <= 0x1p100f)) {
+        first = low < 1.f ? high * low : low;
+        second = low < 1.f ? 1.f : high;
+    }
     return fmaf(c * first, second, sum);
 }
 
@@ -105,7 +114,7 @@ __host__ __device__ constexpr int mg_smem_bytes(int cols, int chunk_blocks, int 
 // Blocks [blk0, blk0 + pad_blk) of the vectors to shared memory, those from n_blk on as zeros: four
 // threads per block, eight elements each, the loads of a few such pieces in flight.  `between` runs
 // behind the first loads: what it starts overlaps their latency.  Whether one of this thread's blocks
-// has a scale from 2^100 on is returned.
+// is far (see mx_scaled) is returned; a block of zeros is not.
 template <int VT, typename F>
 __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float* vscale, int column, int blk0, int n_blk,
                                          int pad_blk, int tid, F&& between) {
@@ -113,7 +122,7 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
     constexpr int kWords = VT == kSrcF32 ? 8 : VT == kSrcMxfp4 ? 1 : 4;   // of eight elements
     constexpr int kBatch = VT == kSrcF32 ? 2 : 4, kStep = kMgThreads / 4;
     const int q = tid & 3, pieces = a.nv * pad_blk;
-    bool begun = false, large = false;
+    bool begun = false, far = false;
     for (int base = 0; base < pieces; base += kBatch * kStep) {
         uint32_t raw[kBatch][kWords];
         uint32_t sb[kBatch];
@@ -160,6 +169,7 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
             if constexpr (VT == kSrcMxfp4) {
                 mx_decode8(raw[u][0], hi);
                 sv = mx_scale_value(sb[u]);
+                far |= sv >= 0x1p100f;
             } else {
                 float x[8];
                 uint32_t top = 0u;
@@ -175,6 +185,7 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
                 const uint32_t f = min(268u - (top >> 23), 253u);   // exponent field of the factor
                 const float factor = __uint_as_float(f << 23);
                 sv = __uint_as_float((254u - f) << 23);
+                far |= sv >= 0x1p100f || (sv < 0x1p-124f && top != 0u);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     unsigned short h[2], l[2];
@@ -189,7 +200,6 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
                     lo[k] = l[0] | ((uint32_t)l[1] << 16);
                 }
             }
-            large |= sv >= 0x1p100f;
             if (i < pieces) {
                 __half* d = vec + (long long)n * kParts * column + b * kMxBlock + q * 8;
                 *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -198,7 +208,7 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
             }
         }
     }
-    return large;
+    return far;
 }
 
 // Four or eight columns.  A lane takes 16 bytes of a row, one block; columns 2 t and 2 t + 1 of a product
@@ -235,6 +245,7 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
     const int chunks = (a.blocks + a.chunk_blocks - 1) / a.chunk_blocks;
     // warps over columns (wk of them) and tasks (wr of them)
     const int wk = a.col_warps, wr = kMgWarps / wk, my_k = warp & (wk - 1), my_r = warp / wk;
+    bool far = false;                                  // the chunk in shared memory has a block that mx_scaled asks about
     for (int first = 0; first < tasks; first += a.slots) {
         const int n_tasks = min(a.slots, tasks - first);
         for (int ch = 0; ch < chunks; ++ch) {
@@ -278,8 +289,9 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
             // the vector chunk: four threads per block, eight elements each
             if (ch > 0 || first > 0 ? chunks > 1 : true) {
                 if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
-                mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, tiles * 4, tid, [] {});
-                __syncthreads();
+                far = mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, tiles * 4, tid, [] {});
+                if constexpr (VT == kSrcF16) __syncthreads();
+                else far = __syncthreads_or(far);
             }
 
             // the products
@@ -332,8 +344,8 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
                         const float sv = p < a.nv ? vscale[p * a.chunk_blocks + b] : 0.f;
 #pragma unroll
                         for (int r = 0; r < R; ++r) {
-                            acc[r][0][p] = mx_scaled<VT>(c[r][0] + c[r][1], sv, sw[r].x, acc[r][0][p]);
-                            acc[r][1][p] = mx_scaled<VT>(c[r][2] + c[r][3], sv, sw[r].y, acc[r][1][p]);
+                            acc[r][0][p] = mx_scaled<VT>(c[r][0] + c[r][1], sv, sw[r].x, acc[r][0][p], far);
+                            acc[r][1][p] = mx_scaled<VT>(c[r][2] + c[r][3], sv, sw[r].y, acc[r][1][p], far);
                         }
                     } else {
 #pragma unroll
@@ -342,8 +354,8 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
                             const float sv = n < a.nv ? vscale[n * a.chunk_blocks + b] : 0.f;
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
-                                acc[r][0][n] = mx_scaled<VT>(c[r][e], sv, sw[r].x, acc[r][0][n]);
-                                acc[r][1][n] = mx_scaled<VT>(c[r][2 + e], sv, sw[r].y, acc[r][1][n]);
+                                acc[r][0][n] = mx_scaled<VT>(c[r][e], sv, sw[r].x, acc[r][0][n], far);
+                                acc[r][1][n] = mx_scaled<VT>(c[r][2 + e], sv, sw[r].y, acc[r][1][n], far);
                             }
                         }
                     }
@@ -490,7 +502,7 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
     }
     __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    bool ok = true, large = false;                   // large: c x sv could overflow, see mx_scaled
+    bool ok = true, far = false;                     // far: see mx_scaled
     int used = 0;                                    // slots read so far, over all chunks
     int filled = 0, lost = 0;                        // slots asked for, and read when a wait gave up
     for (int first = 0; first < tasks; first += a.slots) {
@@ -544,10 +556,10 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
             };
             if (ch > 0 || first > 0 ? chunks > 1 : true) {
                 if (ch > 0 || first > 0) __syncthreads();   // the previous chunk's readers are done
-                large = mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, spans * 8 * kMrLines, tid, begin);
+                far = mg_stage<VT>(a, vec, vscale, column, blk0, n_blk, spans * 8 * kMrLines, tid, begin);
                 if (steps > 0) load_scales();
                 if constexpr (VT == kSrcF16) __syncthreads();
-                else large = __syncthreads_or(large);
+                else far = __syncthreads_or(far);
             } else {
                 begin();
                 if (steps > 0) load_scales();
@@ -614,13 +626,8 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
                             const float2 sw = mx_scale_pair(s[l][r]);
                             const float c0 = kParts == 2 ? c[r][0][0] + c[r][COLS - 1][0] : c[r][n][0];
                             const float c1 = kParts == 2 ? c[r][0][3] + c[r][COLS - 1][3] : c[r][n][3];
-                            if (VT != kSrcF16 && large) {
-                                acc[r][n] = mx_scaled<VT>(c0, sv.x, sw.x, acc[r][n]);
-                                acc[r][n] = mx_scaled<VT>(c1, sv.y, sw.y, acc[r][n]);
-                            } else {
-                                acc[r][n] = fmaf(c0 * sv.x, sw.x, acc[r][n]);
-                                acc[r][n] = fmaf(c1 * sv.y, sw.y, acc[r][n]);
-                            }
+                            acc[r][n] = mx_scaled<VT>(c0, sv.x, sw.x, acc[r][n], far);
+                            acc[r][n] = mx_scaled<VT>(c1, sv.y, sw.y, acc[r][n], far);
                         }
                     }
                 }

@@ -290,6 +290,40 @@ def test_gemv_large_values_times_small_scales_and_the_reverse(M, N, batch, vecto
     assert bool(((got - wide @ m.T).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("vector,up", [("bf16", -130), ("fp32", -130), ("fp32", -140), ("fp32", -148)])
+@pytest.mark.parametrize("M,N,batch", [(40, 256, 1), (40, 300, 1), (300, 30000, 1), (40, 256, 2), (40, 300, 5), (40, 256, 8)])
+def test_gemv_subnormal_vectors_times_large_scales(M, N, batch, vector, up):
+    # blocks of subnormal elements (steps of 2^-133 and 2^-149), against a matrix that makes ordinary numbers of them.  Such a
+    # block is taken to FP16 without a rounding where its largest element is below 2^-127: the factor is 2^126, so the
+    # elements are multiples of 2^-23 below 1/2, which two FP16 hold (BF16: multiples of 2^-7, one does)
+    v = (values(batch, N, 2, torch.float32, spread=0.0).clamp(-2, 2).double() * 2.0 ** up).to(DTYPES[vector])
+    assert bool((v != 0).any())
+    codes, scales = O.quantise(values(M, N, 3, spread=0.0).double() * 2.0 ** 120)
+    m, wide = O.dequantise(codes, scales, N), v.double()
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N)).double()
+    assert bool(((got - wide @ m.T).abs() <= gemv_bound(m, wide, False)).all())
+
+
+@pytest.mark.parametrize("batch", [1, 2, 5])
+def test_gemv_one_element_at_the_far_ends(batch):
+    # every row one code, every result one product: both factors' order must lose nothing that the result could hold
+    N = 96
+    exponents = [-149, -140, -126, -113, -112, -60, 0, 60, 113, 127]
+    v = torch.zeros(len(exponents) * batch, N, device="cuda", dtype=torch.float64)
+    for i, e in enumerate(exponents):
+        v[i * batch:(i + 1) * batch, 40] = 2.0 ** e
+        v[i * batch:(i + 1) * batch, 5] = 2.0 ** -e if e not in (-149, -140) else 1.0   # the far end in another block
+    v = v.float()
+    codes = torch.zeros(255, N // 2, dtype=torch.uint8, device="cuda")
+    codes[:, 20] = 1                                   # 0.5 at column 40
+    scales = torch.full((255, N // 32), 127, dtype=torch.uint8, device="cuda")
+    scales[:, 1] = torch.arange(255, device="cuda").to(torch.uint8)
+    want = v.double() @ O.dequantise(codes, scales, N).T
+    for i in range(len(exponents)):
+        got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v[i * batch:(i + 1) * batch], (255, N))
+        assert torch.equal(got, want[i * batch:(i + 1) * batch].float())        # powers of two, rounded once at FP32's ends
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 def test_several_vectors_infinite_where_the_matrix_is_nan_elsewhere(dtype):
     M, N = 9000, 4096
