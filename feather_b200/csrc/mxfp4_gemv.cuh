@@ -38,6 +38,8 @@
 // 4096 x 4096 4.6, 256 x 2048 3.0; FP32 at 16384 x 16384 31.7, two FP16 vectors 34.5.  The first
 // version (tiles of 16 x 128 loaded to registers, as the many-column kernel still does) took 43.4.
 #pragma once
+#include <type_traits>
+
 #include "attention_tc.cuh"   // tensor-map copies
 #include "gemv_common.cuh"
 #include "mxfp4_codec.cuh"
@@ -72,10 +74,11 @@ __device__ __forceinline__ float2 mx_scale_pair(uint32_t s) {
 //   else their product, if the smaller one is below 1 (2^-27 .. 2^127, exact);
 //   else the smaller first.
 // (2^124 in the vector against 2^-60 in the matrix, 2^-149 against 2^127.)  Only such vectors pay:
-// FP32 at 16384 x 16384 31.7 us, some such order throughout 33.1, never 31.5.
-template <int VT>
-__device__ __forceinline__ float mx_scaled(float c, float sv, float sw, float sum, bool far) {
-    if (VT == kSrcF16 || !far) return fmaf(c * sv, sw, sum);
+// FP32 at 16384 x 16384 31.7 us, some such order throughout 33.1, never 31.5.  The many-column kernel,
+// short of registers, has its loop twice: 2048 x 4096 x 8 BF16 10.5 us, asked at every product 10.95.
+template <bool FAR>
+__device__ __forceinline__ float mx_scaled(float c, float sv, float sw, float sum) {
+    if constexpr (!FAR) return fmaf(c * sv, sw, sum);
     float low, high;                                 // a NaN scale stays one
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(sv), "f"(sw));
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(high) : "f"(sv), "f"(sw));
@@ -299,7 +302,7 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
             float acc[R][2][kAcc];
             int tile = 0, task = my_r;
             const bool diag = (g >> 1) == t;        // this lane's column belongs to its own block
-            auto multiply = [&](int buf) {
+            auto multiply = [&](int buf, auto far) {
                 if (tile == 0) {
 #pragma unroll
                     for (int r = 0; r < R; ++r)
@@ -344,8 +347,8 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
                         const float sv = p < a.nv ? vscale[p * a.chunk_blocks + b] : 0.f;
 #pragma unroll
                         for (int r = 0; r < R; ++r) {
-                            acc[r][0][p] = mx_scaled<VT>(c[r][0] + c[r][1], sv, sw[r].x, acc[r][0][p], far);
-                            acc[r][1][p] = mx_scaled<VT>(c[r][2] + c[r][3], sv, sw[r].y, acc[r][1][p], far);
+                            acc[r][0][p] = mx_scaled<far>(c[r][0] + c[r][1], sv, sw[r].x, acc[r][0][p]);
+                            acc[r][1][p] = mx_scaled<far>(c[r][2] + c[r][3], sv, sw[r].y, acc[r][1][p]);
                         }
                     } else {
 #pragma unroll
@@ -354,8 +357,8 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
                             const float sv = n < a.nv ? vscale[n * a.chunk_blocks + b] : 0.f;
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
-                                acc[r][0][n] = mx_scaled<VT>(c[r][e], sv, sw[r].x, acc[r][0][n], far);
-                                acc[r][1][n] = mx_scaled<VT>(c[r][2 + e], sv, sw[r].y, acc[r][1][n], far);
+                                acc[r][0][n] = mx_scaled<far>(c[r][e], sv, sw[r].x, acc[r][0][n]);
+                                acc[r][1][n] = mx_scaled<far>(c[r][2 + e], sv, sw[r].y, acc[r][1][n]);
                             }
                         }
                     }
@@ -380,15 +383,19 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
                     task += wr;
                 }
             };
-            for (int i = 0; i < steps; i += kBuf) {
+            auto walk = [&](auto far) {
+                for (int i = 0; i < steps; i += kBuf) {
 #pragma unroll
-                for (int u = 0; u < kBuf; ++u) {
-                    if (i + u < steps) {
-                        if (i + u + kBuf - 1 < steps) load((u + kBuf - 1) % kBuf);
-                        multiply(u);
+                    for (int u = 0; u < kBuf; ++u) {
+                        if (i + u < steps) {
+                            if (i + u + kBuf - 1 < steps) load((u + kBuf - 1) % kBuf);
+                            multiply(u, far);
+                        }
                     }
                 }
-            }
+            };
+            if (VT != kSrcF16 && far) walk(std::true_type{});
+            else walk(std::false_type{});
         }
         __syncthreads();
         for (int i = tid; i < n_tasks * a.nv * 16 * R; i += kMgThreads) {
@@ -626,8 +633,13 @@ mx_gemv_ring_kernel(const __grid_constant__ CUtensorMap map, const MxGemvArgs a)
                             const float2 sw = mx_scale_pair(s[l][r]);
                             const float c0 = kParts == 2 ? c[r][0][0] + c[r][COLS - 1][0] : c[r][n][0];
                             const float c1 = kParts == 2 ? c[r][0][3] + c[r][COLS - 1][3] : c[r][n][3];
-                            acc[r][n] = mx_scaled<VT>(c0, sv.x, sw.x, acc[r][n], far);
-                            acc[r][n] = mx_scaled<VT>(c1, sv.y, sw.y, acc[r][n], far);
+                            if (VT != kSrcF16 && far) {
+                                acc[r][n] = mx_scaled<true>(c0, sv.x, sw.x, acc[r][n]);
+                                acc[r][n] = mx_scaled<true>(c1, sv.y, sw.y, acc[r][n]);
+                            } else {
+                                acc[r][n] = mx_scaled<false>(c0, sv.x, sw.x, acc[r][n]);
+                                acc[r][n] = mx_scaled<false>(c1, sv.y, sw.y, acc[r][n]);
+                            }
                         }
                     }
                 }
