@@ -363,6 +363,36 @@ def test_gemm(M, N, batch, dtype):
     assert torch.equal(got, fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N), out_dtype=DTYPES[dtype]))
 
 
+def random_packed(rows, n, seed):
+    """Codes and scales of whole blocks, drawn directly."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randint(0, 256, (rows, n // 2), generator=gen, device="cuda").to(torch.uint8),
+            torch.randint(120, 134, (rows, n // 32), generator=gen, device="cuda").to(torch.uint8))
+
+
+@pytest.mark.parametrize("M,N,batch", [(57001, 96, 16), (57000, 2080, 5), (57000, 96, 20), (57001, 96, 64), (57000, 2080, 40),
+                                       (57000, 96, 100), (57001, 1056, 128), (20000, 2080, 384), (20001, 2080, 384), (20000, 2080, 672),
+                                       (20001, 2080, 672), (20000, 1056, 672), (19980, 96, 700), (20004, 2080, 700)])
+def test_gemm_several_tiles_per_cta(M, N, batch):
+    # more than three tiles of 128 rows for each of 148 SMs, for every width of tile (16, 32, 64, 128 and 224 rows of x): the
+    # rings, the scale groups (an odd number of them where N is 2080), the two accumulators and the pieces of the result go
+    # on from tile to tile; rows of the result on and off the 16-byte grid; the last tiles ragged both ways
+    codes, scales = random_packed(M, N, M + N)
+    x, x_scales = random_packed(batch, N, 5 * M + N)
+    m, w = O.dequantise(codes, scales, N), O.dequantise(x, x_scales, N)
+    want, size = w @ m.T, w.abs() @ m.abs().T
+    del m
+    for dtype in DTYPES.values():
+        out = torch.full((batch + 1, M), 7.0, dtype=dtype, device="cuda")
+        got = fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N), out_dtype=dtype, out=out[:batch])
+        bound = size * (math.ceil(N / 64) + 1) * 2.0 ** -22 + want.abs() * torch.finfo(dtype).eps / 2 * 1.001 + torch.finfo(dtype).tiny
+        top = torch.finfo(dtype).max                   # FP16 overflows where the value does
+        err = (got.double().clamp(-top, top) - want.clamp(-top, top)).abs()
+        assert bool((err <= bound).all()), (err / bound).max()
+        assert bool((out[batch] == 7.0).all())
+        assert torch.equal(got, fb.gemm_mxfp4_acc_fp32_gpu(codes, scales, x, x_scales, (M, N), out_dtype=dtype))
+
+
 def test_gemm_every_place_and_scale_is_its_own():
     # one element and one scale at a time: a row or a scale in the wrong place shows as a wrong number
     M, N, batch = 256, 512, 256
