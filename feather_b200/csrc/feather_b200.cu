@@ -1066,14 +1066,19 @@ static bool mx_wants_digits(long long M, long long N, int batch, int v_dtype) {
     return cols > 2 && N > 0 && M >= (((80ll << 20) + cols - 1) / cols + N - 1) / N;   // cols M N >= 80 M
 }
 
-// Tiles of 224 or of 128 rows of x: those whose waves take less, a wave of the wide ones taking
-// 1.5 times as long (measured at 16384 x 8192 x 4096: 219 and 350 us for 17 and 28 waves).
-static bool mx_wide_tiles(const MxGemmArgs& a, const DeviceInfo& dev) {
+// Tiles of 224 or of 128 rows of x: those whose waves take less.  A wave costs its stages, a wide one
+// 5/4 of a narrow one, and the result's way out, twice as much for wide tiles and twice for FP32:
+// in quarters of a narrow stage 8 + 4 stages (16 + 5 stages wide), FP32 16 + 4 (32 + 5).  Measured per wave
+// where there are many (us, narrow / wide, 8, 16 and 32 stages): BF16 2.9 / 4.1, 5.4 / 7.1, 10.1 / 13.2; FP32 3.5 /
+// 5.6, 5.7 / 7.8, 10.4 / 13.4.  Both sides (us, narrow / wide, BF16): 8192 x 4096 x 1536 31.3 / 26.9 (6 and 4
+// waves), 8192 x 8192 x 1024 40.6 / 37.6 (4 and 3), 4096 x 2048 x 2048 13.5 / 14.3 (4 and 3), 2048 x 8192 x 2048
+// 22.5 / 25.7 (2 and 2), 16384 x 8192 x 2048 142 / 119 (14 and 9).
+static bool mx_wide_tiles(const MxGemmArgs& a, int out_size, const DeviceInfo& dev) {
     if (a.batch <= 128) return false;
-    const long long tm = (a.M + kGmRows - 1) / kGmRows;
+    const long long tm = (a.M + kGmRows - 1) / kGmRows, stages = (a.blocks + kGmBlocks - 1) / kGmBlocks;
     const long long wide = (tm * ((a.batch + 223) / 224) + dev.sm_count - 1) / dev.sm_count;
     const long long narrow = (tm * ((a.batch + 127) / 128) + dev.sm_count - 1) / dev.sm_count;
-    return 3 * wide < 2 * narrow;
+    return wide * (8 * out_size + 5 * stages) < narrow * (4 * out_size + 4 * stages);
 }
 
 template <int OUT>
@@ -1081,7 +1086,7 @@ static int mx_gemm(const unsigned char* x_codes, const MxGemmArgs& a, const Devi
     return a.batch <= 16    ? mx_gemm_launch<16, OUT, false>(x_codes, a, dev, s)
            : a.batch <= 32  ? mx_gemm_launch<32, OUT, false>(x_codes, a, dev, s)
            : a.batch <= 64  ? mx_gemm_launch<64, OUT, false>(x_codes, a, dev, s)
-           : mx_wide_tiles(a, dev) ? mx_gemm_launch<224, OUT, false>(x_codes, a, dev, s)
+           : mx_wide_tiles(a, OUT == kSrcF32 ? 4 : 2, dev) ? mx_gemm_launch<224, OUT, false>(x_codes, a, dev, s)
                                    : mx_gemm_launch<128, OUT, false>(x_codes, a, dev, s);
 }
 
