@@ -48,6 +48,41 @@ def dequantise(codes: torch.Tensor, scales: torch.Tensor, n: int) -> torch.Tenso
     return (grid[c] * s[..., None]).reshape(rows, -1)[:, :n]
 
 
+def digits(v: torch.Tensor, count: int) -> list[torch.Tensor]:
+    """The rows of ``v`` as ``count`` packed rows each, whose sum they are but for what is left: every
+    one is the quantised remainder of those before it.  float64 values, the first digits first."""
+    left, found = v.double(), []
+    for _ in range(count):
+        found.append(dequantise(*quantise(left), v.shape[1]))
+        left = left - found[-1]
+    return found
+
+
+def digit_bound(v):
+    """Error of single elements that were taken apart into 12 packed rows and added up in FP32.  A row leaves at most a quarter of
+    the block's largest remainder (between 4 and 8 scales: rounding leaves up to 1, saturation up to 2 of 8), so after
+    12 of them 2^-24 of the block's largest element T; the sum from the smallest row on rounds its partial sums, which are
+    at most T/4^d plus what is left, and at last the element: 2^-24 (|v| + T/3).  2^-20 of slack for products of these.
+    Rows end at the smallest scale's half code: 2^-129."""
+    blocks = -(-v.shape[1] // 32)
+    top = torch.nn.functional.pad(v.abs(), (0, blocks * 32 - v.shape[1])).view(v.shape[0], blocks, 32).amax(-1)
+    top = top.repeat_interleave(32, 1)[:, :v.shape[1]]
+    return (2.0 ** -24 * top + 2.0 ** -24 * (v.abs() + top / 3)) * (1 + 2.0 ** -20) + 2.0 ** -129
+
+
+def digit_cases(rows, n, device="cpu"):
+    """Vectors that take many digits: normal ones of very different sizes, all ones in the mantissa (every row saturates and
+    leaves a quarter), those beside small elements, one element far below its block's largest."""
+    gen = torch.Generator(device=device).manual_seed(rows * n)
+    v = torch.randn(rows, n, generator=gen, device=device) * torch.exp2(torch.randint(-30, 30, (rows, n), generator=gen, device=device).float())
+    ones = 1 - 2.0 ** -24
+    v[0] = ones * torch.exp2((torch.arange(n, device=device) // 32 % 7 - 3).float())
+    v[-1] = torch.randn(n, generator=gen, device=device)
+    v[-1, ::2] = -ones
+    v[1, 5::32], v[1, 6::32] = ones, 1.25 * 2.0 ** -20
+    return v
+
+
 def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, layout: str, scale: float = 1.0):
     """float64 (tokens, heads, dim), the rotation written element by element."""
     y = x.double().clone()

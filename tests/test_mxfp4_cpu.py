@@ -186,3 +186,25 @@ if {gone!r}.endswith("RawStream"):
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert done.returncode == 0, done.stderr
+
+
+def added_up(found):
+    """The rows' sum in FP32, the smallest first."""
+    total = found[-1].float()
+    for d in found[-2::-1]:
+        total = total + d.float()
+    return total.double()
+
+
+def test_twelve_digits_are_what_it_takes():
+    v = O.digit_cases(4, 700)
+    wide = v.double()
+    ok = [bool(((added_up(O.digits(v, count)) - wide).abs() <= O.digit_bound(wide)).all()) for count in (10, 11, 12)]
+    assert ok == [False, False, True]
+    found = O.digits(v, 12)
+    found[11] = torch.zeros_like(found[11])                       # a row that is lost, or has its neighbour's scale
+    assert not bool(((added_up(found) - wide).abs() <= O.digit_bound(wide)).all())
+    for lost in (0, 5, 10):
+        found = O.digits(v, 12)
+        found[lost] = 2 * found[lost]
+        assert not bool(((added_up(found) - wide).abs() <= O.digit_bound(wide)).all())

@@ -177,6 +177,54 @@ def test_digits_of_numbers_just_below_powers_of_two():
     assert bool(((got.double() - v.double() @ m.T).abs() <= digits_bound(m, v.double())).all())
 
 
+def single_codes(M, N, seed):
+    """A packed matrix with one code that is not zero per row: (codes, scales, its column, its value)."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    row = torch.arange(M, device="cuda")
+    k = (row * 37 + torch.div(row, N, rounding_mode="floor")) % N
+    code = torch.randint(1, 8, (M,), generator=gen, device="cuda") + 8 * torch.randint(0, 2, (M,), generator=gen, device="cuda")
+    codes = torch.zeros(M, -(-N // 32) * 16, dtype=torch.uint8, device="cuda")
+    codes[row, k // 2] = (code << (4 * (k % 2))).to(torch.uint8)
+    scales = torch.randint(120, 135, (M, -(-N // 32)), generator=gen, device="cuda").to(torch.uint8)
+    grid = torch.tensor(O.VALUES + [-x for x in O.VALUES], dtype=torch.float64, device="cuda")
+    return codes, scales, k, grid[code] * torch.exp2(scales[row, k // 32].double() - 127)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("M,N,batch", [(9000, 4096, 3), (9000, 4096, 8), (9000, 4096, 9), (2500, 5000, 17), (2050, 16384, 4), (57001, 512, 3),
+                                       (57001, 512, 9)])
+def test_digits_hold_every_element(M, N, batch, dtype):
+    # every result one product, so that no other element's error hides a row that is missing.  Matrices in one tile per
+    # cluster and in more than three tiles per SM; batches whose last pass has one vector
+    codes, scales, k, m = single_codes(M, N, M + batch)
+    v = O.digit_cases(batch, N, "cuda").to(DTYPES[dtype])
+    if dtype == "fp16":
+        v = v.clamp(-60000, 60000)
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N)).double()
+    err, bound = (got - v.double()[:, k] * m).abs(), O.digit_bound(v.double())[:, k] * m.abs()
+    assert bool((err <= bound).all()), (err / bound).max()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("batch", [3, 9])
+def test_digits_of_more_tiles_than_sms(batch, dtype):
+    # three and more tiles per SM, the vectors that are not finite repaired in each
+    M, N = 57001, 512
+    codes, scales = random_packed(M, N, batch)
+    scales[33333, 3] = 255
+    m = O.dequantise(codes, scales, N)
+    v = values(batch, N, 4, DTYPES[dtype], spread=2.0)
+    fine = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+    v[batch - 1, 70], v[1, 5], v[1, 300] = float("inf"), -float("inf"), float("inf")
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N))
+    want = v.double() @ m.T
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[want.isinf()].double(), want[want.isinf()])
+    keep = [b for b in range(batch) if b not in (1, batch - 1)]
+    assert torch.equal(got[keep].nan_to_num(7.0), fine[keep].nan_to_num(7.0))
+    err, bound = (got.double() - want)[keep].abs(), digits_bound(m.nan_to_num(0.0), v.double()[keep])
+    assert bool((err <= bound)[want[keep].isfinite()].all())
+
+
 def test_gemv_large():
     M, N = 9000, 16384
     codes, scales = packed(M, N, 3)
