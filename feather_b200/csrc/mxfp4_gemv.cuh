@@ -20,9 +20,12 @@
 //
 // The vector.  A block is scaled by a power of two so that its largest finite element lies in
 // [2^14, 2^15), and rounded to FP16.  FP16, BF16 and packed values are exact but for what lies
-// below FP16's smallest step, 2^-40 of the block's largest element -- less than the FP32 sum
-// keeps.  FP32 values are split in two, x = hi + lo, each rounded to nearest: at most 2^-24 of the
-// element (one FP32 rounding) or that same 2^-40.  The block sum (FP32) is multiplied by the
+// below FP16's smallest step, half of which is 2^-39 of the block's largest element -- less than
+// the FP32 sum keeps.  FP32 values are split in two, x = hi + lo, each rounded to nearest: 2 x 11 bits
+// and lo's sign leave at most 2^-23 of the element (a quarter of random ones lose more than 2^-24, what
+// rounding to FP32 would), or that same 2^-39; a third part would cost a third column.  Blocks below
+// 2^-112 stay below 2^14 (the factor ends at 2^126) and lose nothing more by it: all FP32 numbers are
+// multiples of 2^-149, there 2^-23.  The block sum (FP32) is multiplied by the
 // vector block's power of two and by the matrix block's, the second time in the FMA that adds it.
 //
 // Two kernels.  mx_gemv_ring_kernel: one or two columns per block, any size (below).

@@ -41,7 +41,12 @@ def gemv_mxfp4_acc_fp32_gpu(m_codes: torch.Tensor, m_scales: torch.Tensor, v: to
     ``m_codes``, ``m_scales``: what ``pack_mxfp4_tensor`` returns for an ``(M, N)`` matrix.
     ``v``: a contiguous float16, bfloat16 or float32 tensor of shape ``(N,)`` or ``(batch, N)``, or
     packed codes together with ``v_scales``.  Up to eight vectors go through one pass over the
-    matrix (four float32 ones where it is small); at most 64."""
+    matrix (four float32 ones where it is small); at most 64.
+
+    What a vector's elements are used with: packed ones exactly; one or two vectors, or more on small
+    matrices, to ``2 ** -23`` of the element (float32; float16 and bfloat16 exactly) or ``2 ** -39`` of the largest in its
+    32-element block; more on large matrices (three 16-bit or two float32 ones, from ``columns * M * N = 80 * 2 ** 20`` on,
+    a float32 vector counting as two columns) to ``2 ** -24`` of the largest in the block or ``2 ** -129``."""
     M, N = _shape(m_shape)
     idx = as_packed(m_codes, m_scales, M, N, "m")
     if not isinstance(v, torch.Tensor):

@@ -538,6 +538,11 @@ int feather_decode_mxfp4(const uint8_t* codes, const uint8_t* scales, void* dst,
  *   v         batch x N values of v_dtype, contiguous, or FEATHER_SRC_MXFP4:
  *             packed codes with v_scales (ignored otherwise)
  *   out       batch x M floats
+ * Elements of v are used to 2^-23 of themselves (FP32; FP16 and BF16 exactly) or
+ * 2^-39 of the largest in their 32-element block; where a workspace is needed
+ * (three 16-bit or two FP32 vectors on, large matrices) to 2^-24 of the largest in
+ * the block, or 2^-129, and scale products below FP32's normal range may count as
+ * zero.  Packed vectors are used exactly, several of them as by feather_gemm_mxfp4.
  *   workspace feather_gemv_mxfp4_workspace_bytes(M, N, batch, v_dtype) bytes, 16-byte
  *             aligned, contents irrelevant; may be NULL where that is 0.  Calls
  *             that can overlap need one each
@@ -550,7 +555,8 @@ int64_t feather_gemv_mxfp4_workspace_bytes(int64_t M, int64_t N, int batch, int 
 /*
  * out[b][r] = sum_j value(m[r][j]) * value(x[b][j]), both operands packed
  * MXFP4, on the tensor cores' microscaled kind; FP32 accumulation, one rounding
- * to out_dtype (FEATHER_SRC_F16 / _F32 / _BF16).  No counterpart in the reference.
+ * to out_dtype (FEATHER_SRC_F16 / _F32 / _BF16); a product of scales below FP32's
+ * normal range may count as zero.  No counterpart in the reference.
  *   out       batch x M values
  */
 int feather_gemm_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const uint8_t* x_codes,

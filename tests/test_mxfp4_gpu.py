@@ -191,6 +191,28 @@ def single_codes(M, N, seed):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("M,N,batch", [(600, 512, 1), (600, 520, 1), (600, 512, 2), (600, 520, 2), (600, 512, 4), (600, 520, 8)])
+def test_gemv_holds_every_element(M, N, batch, dtype):
+    # every result one product.  A block's largest element is brought to [2^14, 2^15) and rounded to FP16, whose smallest step
+    # is 2^-24: 2^-39 of the largest element at most, 16-bit vectors lose nothing else.  An FP32 element is the sum of two FP16
+    # numbers of 11 bits: of an element from 2^e on the first leaves at most 2^(e - 11), and rounding that to 11 bits at most
+    # 2^(e - 23) (1 + 2^-12 + 2^-23 loses that).  Then one FP32 rounding, of the two parts' sum.
+    codes, scales, k, m = single_codes(M, N, M + batch)
+    v = O.digit_cases(max(batch, 2), N, "cuda")[:batch]
+    v[0, 64:96] = 1 + 2.0 ** -12 + 2.0 ** -23
+    v = v.to(DTYPES[dtype])
+    if dtype == "fp16":
+        v = v.clamp(-60000, 60000)
+    wide = v.double()
+    blocks = -(-N // 32)
+    top = torch.nn.functional.pad(wide.abs(), (0, blocks * 32 - N)).view(batch, blocks, 32).amax(-1).repeat_interleave(32, 1)[:, :N]
+    bound = 2.0 ** -39 * top + (wide.abs() * (2.0 ** -23 + 2.0 ** -24) if dtype == "fp32" else 0)
+    got = fb.gemv_mxfp4_acc_fp32_gpu(codes, scales, v, (M, N)).double()
+    err = (got - wide[:, k] * m).abs()
+    assert bool((err <= bound[:, k] * m.abs()).all()), (err / (bound[:, k] * m.abs())).max()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("M,N,batch", [(9000, 4096, 3), (9000, 4096, 8), (9000, 4096, 9), (2500, 5000, 17), (2050, 16384, 4), (57001, 512, 3),
                                        (57001, 512, 9)])
 def test_digits_hold_every_element(M, N, batch, dtype):
