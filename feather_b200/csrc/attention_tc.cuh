@@ -148,6 +148,11 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
 }
+// The same box into L2 only.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
+}
 // Instruction descriptors: FP32 accumulator (bits 4-5 = 1), operand formats (bits 7-9 and
 // 10-12: E5M2 = 1 for kind::f8f6f4, FP16 = 0 for kind::f16), B MN-major (bit 16), N / 8 (bits
 // 17-22), M / 16 (bits 24-28).

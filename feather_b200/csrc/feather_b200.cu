@@ -916,7 +916,7 @@ static int mx_decode_launch(const unsigned char* codes, const unsigned char* sca
 
 template <int VT, int COLS>
 static int mx_gemv_many(MxGemvArgs a, const DeviceInfo& dev, cudaStream_t s) {
-    auto kernel = mx_gemv_many_kernel<VT, COLS, 1>;
+    auto kernel = mx_gemv_many_kernel<VT, COLS>;
     constexpr int kMostBlocks = (kMgVecHalfs / COLS / kMxBlock) & ~3;
     a.chunk_blocks = a.blocks < kMostBlocks ? (a.blocks + 3) & ~3 : kMostBlocks;
     static std::atomic<unsigned long long> configured{0};
@@ -989,7 +989,6 @@ template <int VT>
 static int mx_gemv(MxGemvArgs a, int batch, const DeviceInfo& dev, cudaStream_t s) {
     constexpr int kParts = VT == kSrcF32 ? 2 : 1;
     const int most = 8 / kParts;
-    const long long v_bytes = VT == kSrcMxfp4 ? 16ll * a.blocks : a.N * (VT == kSrcF32 ? 4 : 2);
     for (int b = 0; b < batch; b += most) {
         a.nv = batch - b < most ? batch - b : most;
         const int cols = a.nv * kParts;
@@ -998,8 +997,7 @@ static int mx_gemv(MxGemvArgs a, int batch, const DeviceInfo& dev, cudaStream_t 
                        : cols <= 4 ? mx_gemv_cols<VT, 4>(a, dev, s)
                                    : mx_gemv_cols<VT, 8>(a, dev, s);
         if (st != FEATHER_OK) return st;
-        a.v = reinterpret_cast<const unsigned char*>(a.v) + most * v_bytes;
-        if (VT == kSrcMxfp4) a.v_scales += (long long)most * a.blocks;
+        a.v = reinterpret_cast<const typename MxElem<VT>::type*>(a.v) + most * a.N;
         a.out += most * a.M;
     }
     return FEATHER_OK;
@@ -1828,7 +1826,7 @@ int feather_gemv_mxfp4(const uint8_t* m_codes, const uint8_t* m_scales, const vo
         case FEATHER_SRC_F16: return mx_gemv<kSrcF16>(a, batch, *dev, s);
         case FEATHER_SRC_F32: return mx_gemv<kSrcF32>(a, batch, *dev, s);
         case FEATHER_SRC_BF16: return mx_gemv<kSrcBF16>(a, batch, *dev, s);
-        default: return mx_gemv<kSrcMxfp4>(a, batch, *dev, s);
+        default: a.nv = 1; return mx_gemv_cols<kSrcMxfp4, 1>(a, *dev, s);
     }
 }
 

@@ -110,12 +110,6 @@ __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.w
 template <int N>
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A box into L2 only.
-__device__ __forceinline__ void gm_prefetch_2d(const CUtensorMap* map, int x, int y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
-}
-
 // Host side: the result as a 2-D tensor map with boxes of 32 of m x `piece` rows of x.
 inline bool gm_make_out_map(CUtensorMap* map, void* out, int out_size, bool bf16, long long M, long long batch, int piece) {
     const AtcEncodeTiled encode = atc_encoder();
@@ -347,7 +341,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_m, const __grid_constant_
     // land in L2 too).  16384 x 16384 x 16 27.0 -> 25.6 us.
     if (!DIGITS && warp == 0 && lane == 0 && tile0 < n_tiles)
         for (int k = 0; k < min(L::kStages, n_step); ++k)
-            gm_prefetch_2d(&map_m, (k_begin + k) * kGmBox, (tile0 / g.tiles_x) * kGmRows);
+            tma_prefetch_2d(&map_m, (k_begin + k) * kGmBox, (tile0 / g.tiles_x) * kGmRows);
     __syncwarp();
     // Operands and result may be the previous kernel's -- but for the matrix of dense vectors: that
     // kernel is mx_digits_kernel, which starts this one when all before it is done.

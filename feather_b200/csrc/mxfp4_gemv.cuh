@@ -96,8 +96,8 @@ __device__ __forceinline__ float mx_scaled(float c, float sv, float sw, float su
 struct MxGemvArgs {
     const unsigned char* codes;
     const unsigned char* scales;
-    const void* v;                   // nv vectors, N elements (or packed rows) apart
-    const unsigned char* v_scales;   // packed vectors only
+    const void* v;                   // nv vectors, N elements apart
+    const unsigned char* v_scales;   // of a packed vector (one per launch)
     float* out;                      // nv x M
     long long M, N;
     int blocks;                      // per row
@@ -142,9 +142,8 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
             sb[u] = 127u;
             if (b >= n_blk) continue;
             if constexpr (VT == kSrcMxfp4) {
-                const long long at = (long long)n * a.blocks + blk0 + b;
-                raw[u][0] = __ldg(reinterpret_cast<const uint32_t*>(a.v) + at * 4 + q);
-                sb[u] = __ldg(a.v_scales + at);
+                raw[u][0] = __ldg(reinterpret_cast<const uint32_t*>(a.v) + (long long)(blk0 + b) * 4 + q);   // there is one
+                sb[u] = __ldg(a.v_scales + blk0 + b);
             } else {
                 typedef typename MxElem<VT>::type E;
                 const E* p = reinterpret_cast<const E*>(a.v) + (long long)n * a.N + e0;
@@ -219,14 +218,14 @@ __device__ __forceinline__ bool mg_stage(const MxGemvArgs& a, __half* vec, float
 
 // Four or eight columns.  A lane takes 16 bytes of a row, one block; columns 2 t and 2 t + 1 of a product
 // are two vectors, or the halves of an FP32 one, for lane t's block.  VT: type of the vector
-// (kSrc...); COLS: columns, an FP32 vector takes two; R: 16-row groups a warp multiplies with the
-// same vector registers.
-template <int VT, int COLS, int R>
+// (kSrc..., not a packed one); COLS: columns, an FP32 vector takes two.
+template <int VT, int COLS>
 __global__ void __launch_bounds__(kMgThreads, 1)
 mx_gemv_many_kernel(const MxGemvArgs a) {
     constexpr int kParts = VT == kSrcF32 ? 2 : 1;      // columns per vector
     constexpr int kAcc = COLS / kParts;                // vectors a launch can take
-    constexpr int P = (COLS + 1) / 2;                  // products per 16 codes
+    constexpr int P = COLS / 2;                        // products per 16 codes
+    static_assert(COLS % 2 == 0 && VT != kSrcMxfp4, "two columns to a product");
     constexpr int kBuf = 3;                            // tiles in flight
     extern __shared__ __align__(16) unsigned char mg_smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -241,9 +240,8 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
 
     const long long groups = (a.M + 15) / 16;
     const long long g_begin = groups * blockIdx.x / gridDim.x, g_end = groups * (blockIdx.x + 1) / gridDim.x;
-    const int my_groups = (int)(g_end - g_begin);
-    const int tasks = (my_groups + R - 1) / R;
-    const int my_rows = (int)min(a.M - g_begin * 16, (long long)my_groups * 16);
+    const int tasks = (int)(g_end - g_begin);          // a 16-row group each
+    const int my_rows = (int)min(a.M - g_begin * 16, (long long)tasks * 16);
     const uint4* codes = reinterpret_cast<const uint4*>(a.codes) + g_begin * 16 * a.blocks;
     const unsigned char* scales = a.scales + g_begin * 16 * a.blocks;
     if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0u;
@@ -265,27 +263,23 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
             // count from the CTA's first row in 32 bits.  Rows past the last are the last row again
             // and blocks past the row's end its last block again: the former are not stored, the
             // latter meet a vector of zeros.
-            uint4 m[kBuf][R][2];
-            uint32_t s[kBuf][R][2];
-            uint32_t row_at[R][2];
+            uint4 m[kBuf][2];
+            uint32_t s[kBuf][2];
+            uint32_t row_at[2];
             int l_tile = 0, l_task = my_r;
             auto load = [&](int buf) {
                 if (l_tile == 0) {
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            row_at[r][h] = (uint32_t)min(((first + l_task) * R + r) * 16 + g + 8 * h, my_rows - 1) * (uint32_t)a.blocks;
+                    for (int h = 0; h < 2; ++h)
+                        row_at[h] = (uint32_t)min((first + l_task) * 16 + g + 8 * h, my_rows - 1) * (uint32_t)a.blocks;
                 }
                 const uint32_t blk = (uint32_t)(blk0 + min((tile_begin + l_tile) * 4 + t, n_blk - 1));
 #pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t at = row_at[r][h] + blk;
-                        m[buf][r][h] = ldg_stream(codes + at);
-                        s[buf][r][h] = __ldg(scales + at);
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t at = row_at[h] + blk;
+                    m[buf][h] = ldg_stream(codes + at);
+                    s[buf][h] = __ldg(scales + at);
+                }
                 if (++l_tile == my_tiles) l_tile = 0, l_task += wr;
             };
 #pragma unroll
@@ -302,86 +296,67 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
 
             // the products
             const int n_col = a.nv * kParts;
-            float acc[R][2][kAcc];
+            float acc[2][kAcc];
             int tile = 0, task = my_r;
             const bool diag = (g >> 1) == t;        // this lane's column belongs to its own block
             auto multiply = [&](int buf, auto far) {
                 if (tile == 0) {
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int n = 0; n < kAcc; ++n) acc[r][h][n] = 0.f;
+                        for (int n = 0; n < kAcc; ++n) acc[h][n] = 0.f;
                 }
                 const int b = (tile_begin + tile) * 4 + t;      // block inside the chunk
-                float2 sw[R];
+                const float2 sw = mx_scale_pair(s[buf][0] | (s[buf][1] << 8));
+                uint32_t x[2][4][4];                    // decoded once, multiplied with every pair of columns
 #pragma unroll
-                for (int r = 0; r < R; ++r) sw[r] = mx_scale_pair(s[buf][r][0] | (s[buf][r][1] << 8));
-                uint32_t x[R][2][4][4];                 // decoded once, multiplied with every pair of columns
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        mx_decode8(m[buf][r][h].x, x[r][h][0]);
-                        mx_decode8(m[buf][r][h].y, x[r][h][1]);
-                        mx_decode8(m[buf][r][h].z, x[r][h][2]);
-                        mx_decode8(m[buf][r][h].w, x[r][h][3]);
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    mx_decode8(m[buf][h].x, x[h][0]);
+                    mx_decode8(m[buf][h].y, x[h][1]);
+                    mx_decode8(m[buf][h].z, x[h][2]);
+                    mx_decode8(m[buf][h].w, x[h][3]);
+                }
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
                     const int col = 2 * p + (g & 1);
                     const uint4* src = reinterpret_cast<const uint4*>(
                         diag && col < n_col ? reinterpret_cast<const unsigned char*>(vec + col * column + b * kMxBlock) : zeros);
-                    float c[R][4];
-#pragma unroll
-                    for (int r = 0; r < R; ++r) c[r][0] = c[r][1] = c[r][2] = c[r][3] = 0.f;
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const uint4 bv = src[w];
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            mma_f16(c[r], x[r][0][w][0], x[r][1][w][0], x[r][0][w][1], x[r][1][w][1], bv.x, bv.y);
-                            mma_f16(c[r], x[r][0][w][2], x[r][1][w][2], x[r][0][w][3], x[r][1][w][3], bv.z, bv.w);
-                        }
+                        mma_f16(c, x[0][w][0], x[1][w][0], x[0][w][1], x[1][w][1], bv.x, bv.y);
+                        mma_f16(c, x[0][w][2], x[1][w][2], x[0][w][3], x[1][w][3], bv.z, bv.w);
                     }
                     // (a block's sum) x (the vector block's power of two) x (the matrix block's)
                     if constexpr (kParts == 2) {
                         const float sv = p < a.nv ? vscale[p * a.chunk_blocks + b] : 0.f;
-#pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            acc[r][0][p] = mx_scaled<far>(c[r][0] + c[r][1], sv, sw[r].x, acc[r][0][p]);
-                            acc[r][1][p] = mx_scaled<far>(c[r][2] + c[r][3], sv, sw[r].y, acc[r][1][p]);
-                        }
+                        acc[0][p] = mx_scaled<far>(c[0] + c[1], sv, sw.x, acc[0][p]);
+                        acc[1][p] = mx_scaled<far>(c[2] + c[3], sv, sw.y, acc[1][p]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < (COLS > 1 ? 2 : 1); ++e) {
+                        for (int e = 0; e < 2; ++e) {
                             const int n = 2 * p + e;
                             const float sv = n < a.nv ? vscale[n * a.chunk_blocks + b] : 0.f;
-#pragma unroll
-                            for (int r = 0; r < R; ++r) {
-                                acc[r][0][n] = mx_scaled<far>(c[r][e], sv, sw[r].x, acc[r][0][n]);
-                                acc[r][1][n] = mx_scaled<far>(c[r][2 + e], sv, sw[r].y, acc[r][1][n]);
-                            }
+                            acc[0][n] = mx_scaled<far>(c[e], sv, sw.x, acc[0][n]);
+                            acc[1][n] = mx_scaled<far>(c[2 + e], sv, sw.y, acc[1][n]);
                         }
                     }
                 }
                 if (++tile == my_tiles) {
                     // the row's partial sums: over the four lanes, then one slot per warp
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int n = 0; n < kAcc; ++n) {
-                                float x = acc[r][h][n];
-                                x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
-                                x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
-                                if (t == 0 && n < a.nv) {
-                                    float* to = part + ((task * wk + my_k) * a.nv + n) * (16 * R) + r * 16 + h * 8 + g;
-                                    *to = ch == 0 ? x : *to + x;
-                                }
+                        for (int n = 0; n < kAcc; ++n) {
+                            float x = acc[h][n];
+                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+                            x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+                            if (t == 0 && n < a.nv) {
+                                float* to = part + ((task * wk + my_k) * a.nv + n) * 16 + h * 8 + g;
+                                *to = ch == 0 ? x : *to + x;
                             }
+                        }
                     tile = 0;
                     task += wr;
                 }
@@ -401,13 +376,12 @@ mx_gemv_many_kernel(const MxGemvArgs a) {
             else walk(std::false_type{});
         }
         __syncthreads();
-        for (int i = tid; i < n_tasks * a.nv * 16 * R; i += kMgThreads) {
-            const int r = i % (16 * R), n = (i / (16 * R)) % a.nv, task = i / (16 * R * a.nv);
-            const int grp = (first + task) * R + r / 16;
-            const long long row = (g_begin + grp) * 16 + (r & 15);
+        for (int i = tid; i < n_tasks * a.nv * 16; i += kMgThreads) {
+            const int r = i % 16, n = (i / 16) % a.nv, task = i / (16 * a.nv);
+            const long long row = (g_begin + first + task) * 16 + r;
             float x = 0.f;
-            for (int k = 0; k < wk; ++k) x += part[((task * wk + k) * a.nv + n) * (16 * R) + r];
-            if (grp < my_groups && row < a.M) a.out[n * a.M + row] = x;
+            for (int k = 0; k < wk; ++k) x += part[((task * wk + k) * a.nv + n) * 16 + r];
+            if (row < a.M) a.out[n * a.M + row] = x;
         }
         __syncthreads();
     }
@@ -437,10 +411,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
     asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];"
                  ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
 }
 // Host side: rows of whole lines as {128 bytes, rows, lines} with boxes of 16 rows x 2 lines.
 inline bool mr_make_map(CUtensorMap* map, const void* base, long long row_bytes, long long rows) {
