@@ -1057,8 +1057,11 @@ static int mx_scale_align(const void* m_scales, const void* x_scales, int blocks
 }
 
 // Which dense vectors go through the product kernel as digits: three columns of the GEMV kernels
-// or more, times the matrix.  Measured (us, many-column GEMV against digits): 8192^2 x 3 FP16 22.4 / 14.6,
-// 4096^2 x 8 14.8 / 12.1, x 3 9.4 / 10.2, 2048^2 x 8 6.7 / 9.0, 256 x 2048 x 8 6.6 / 9.0.
+// or more, times the matrix.  Measured (us, GEMV kernels / digits; FP16 but where FP32 is said): 2048^2 x 8 6.8 / 8.6, 4096^2
+// x 3 9.1 / 9.1, x 4 9.6 / 9.2, x 8 14.6 / 10.8, 2048 x 8192 x 3 10.3 / 10.1, 8192 x 2048 x 3 9.4 / 8.2, 8192^2 x 3 22.6 / 14.0,
+// two FP32 19.0 / 13.9; 16384^2 x 8 137 / 32.9.  Two columns stay with the ring kernel, which keeps every element to 2^-23 of
+// itself, not of its block: one FP32 and two FP16 vectors 5.3 and 5.8 / 8.8 and 8.9 at 4096^2, 12.3 and 13.4 / 13.8 and 13.9 at
+// 8192^2, and 32.3 and 34.6 / 29.2 at 16384^2, the one size measured at which digits gain more than 5 %.
 static bool mx_wants_digits(long long M, long long N, int batch, int v_dtype) {
     const long long cols = (long long)batch * (v_dtype == FEATHER_SRC_F32 ? 2 : 1);
     return cols > 2 && N > 0 && M >= (((80ll << 20) + cols - 1) / cols + N - 1) / N;   // cols M N >= 80 M
