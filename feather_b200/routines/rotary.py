@@ -84,9 +84,12 @@ def rotary_gpu(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
 
     Returns ``(tokens, heads, dim)`` of ``x``'s type (``out`` may be ``x`` itself where it is
     contiguous), or with ``mode`` "E5M2" / "E4M3" the FP8 words ``(heads, tokens, dim / 4)``: one
-    head's ``result[h]`` is a packed (tokens, dim) matrix.  Words written to ``out`` come back tagged with
-    ``mode`` too, and an ``out`` that carries a tag has it changed.  The angles are computed in 64 bits, so
-    positions far into a context lose nothing."""
+    head's ``result[h]`` is a packed (tokens, dim) matrix.  Words written to ``out`` come back
+    tagged with ``mode`` too, and an ``out`` that carries a tag has it changed.
+
+    The angles are computed in 64 bits, ``|angle| * 2 ** -51`` off at most before the FP32 sine and
+    cosine of what is left of a turn: position ``2 ** 26`` loses nothing, ``2 ** 31`` up to a
+    millionth of a radian."""
     if not (isinstance(x, torch.Tensor) and isinstance(positions, torch.Tensor) and isinstance(inv_freq, torch.Tensor)):
         raise TypeError("x, positions and inv_freq must be torch.Tensors")
     if layout not in LAYOUTS:
